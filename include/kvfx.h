@@ -49,6 +49,9 @@ extern "C" {
 /* Most sequences one kvfx_attention_batch call takes. */
 #define KVFX_MAX_PREFILL_SEQS 32u
 
+/* Slot of a padding token (kvfx_write_rotated): nothing is written for it. */
+#define KVFX_NO_SLOT UINT64_MAX
+
 /* Bits of the per-device status word. */
 #define KVFX_FLAG_BAD_INDEX 1u  /* a slot/block id beyond the cache was skipped */
 #define KVFX_FLAG_TIMEOUT 2u    /* a bounded wait inside a kernel expired        */
@@ -128,6 +131,79 @@ int kvfx_gather_layers(const kvfx_cache* caches, uint32_t num_layers, const uint
  */
 int kvfx_copy_page(const kvfx_cache* cache, uint64_t src_block, uint64_t dst_block,
                    void* stream);
+
+/*
+ * Copies inside the caches of a layer batch (caches, num_layers as for
+ * kvfx_write_layers), one launch for all layers, byte-exact.
+ *   kvfx_copy_pages: page dst_pages[i] = page src_pages[i], i < num_pages, in K
+ *     and V of every layer (the private last pages of a batch of forks).
+ *   kvfx_copy_slots: the rows of slot dst_slots[i] = those of slot
+ *     src_slots[i], every head, K and V of every layer (the kept tokens of an
+ *     eviction, moved together into fresh pages).
+ * The id arrays are device uint64. A source may appear several times; each
+ * destination may appear once, and no destination may be a source of the same
+ * call (what a violation leaves in those pages or slots is undefined). An id
+ * outside the cache is skipped and sets KVFX_FLAG_BAD_INDEX.
+ * No counterpart in the reference, which copies one page of one layer per
+ * call (src/v2/paged_kv_storage.cpp:70-93) and never moves tokens.
+ */
+int kvfx_copy_pages(const kvfx_cache* caches, uint32_t num_layers, const uint64_t* src_pages,
+                    const uint64_t* dst_pages, uint64_t num_pages, void* stream);
+int kvfx_copy_slots(const kvfx_cache* caches, uint32_t num_layers, const uint64_t* src_slots,
+                    const uint64_t* dst_slots, uint64_t num_slots, void* stream);
+
+/*
+ * Rotary positions and the per-head norms of Q and K, as kvfx_write_rotated
+ * applies them. A head's first rotary_dim dimensions are turned in pairs by
+ * the angles of the token's position: pair i is dimensions (i, i +
+ * rotary_dim / 2), or (2i, 2i + 1) when interleaved is 1. Row p of cos_sin
+ * holds position p's rotary_dim / 2 cosines, then its sines.
+ */
+typedef struct kvfx_rotary {
+    const float* cos_sin;    /* device [max_positions][rotary_dim]                 */
+    uint64_t max_positions;
+    uint32_t rotary_dim;     /* even, 2 .. head_size                                */
+    uint32_t interleaved;    /* 0 or 1                                              */
+    const float* q_weight;   /* device [head_size], or NULL: Q heads are not normed */
+    const float* k_weight;   /* device [head_size], or NULL: K heads are not normed */
+    float eps;               /* added to the mean square, >= 0                      */
+    uint32_t reserved;       /* must be 0                                           */
+} kvfx_rotary;
+
+/*
+ * Fills a cos_sin table: angle i of position p is
+ * p * position_scale * base^(-2i / rotary_dim), computed in FP64.
+ * base > 0, position_scale finite.
+ */
+int kvfx_rotary_table(float* cos_sin, uint64_t max_positions, uint32_t rotary_dim, double base,
+                      double position_scale, int device, void* stream);
+
+/*
+ * New tokens' Q, K and V in one pass: K and Q heads are normed (y = x /
+ * sqrt(mean(x^2) + eps) * weight, where weights are given) and rotated, K and
+ * V go to their cache slots as in kvfx_write, and Q goes out in FP32 as the
+ * attention entry points take it. Computed in FP32; K is rounded once.
+ *   q, k, v   : device, the cache's dtype; token t's heads are contiguous
+ *               rows of head_size from q + t * q_stride on (strides in
+ *               elements, at least heads * head_size, so the three may be
+ *               slices of one projection's output); must not overlap the
+ *               cache or q_out
+ *   positions : device uint64[num_tokens], each < max_positions
+ *   slots     : device uint64[num_tokens], pairwise distinct; KVFX_NO_SLOT
+ *               marks a padding token: nothing of it is read or written
+ *   q_out     : device float[num_tokens][q_heads][head_size]
+ * q_heads may be 0 (q and q_out are then not looked at). A token whose slot
+ * or position is out of range is skipped and sets KVFX_FLAG_BAD_INDEX.
+ * Rows of 32, 64, 128 or 256 elements with 16-byte aligned bases and strides,
+ * and a rotary_dim that is a multiple of 16 (8 interleaved), take a kernel of
+ * 16-byte vectors; other shapes an element-wise one.
+ * No counterpart in the reference, whose write takes K and V as they are
+ * (src/v2/paged_kv_write.cu:101-139).
+ */
+int kvfx_write_rotated(const kvfx_cache* cache, const kvfx_rotary* rotary, const void* q, const void* k,
+                       const void* v, uint64_t q_stride, uint64_t k_stride, uint64_t v_stride,
+                       uint32_t q_heads, const uint64_t* positions, const uint64_t* slots,
+                       uint64_t num_tokens, float* q_out, void* stream);
 
 /*
  * Batch decode PagedAttention: one last-position query per sequence.

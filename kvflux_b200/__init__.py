@@ -37,6 +37,7 @@ KVFX_F16, KVFX_BF16, KVFX_F32 = 0, 1, 2
 KVFX_FLAG_BAD_INDEX, KVFX_FLAG_TIMEOUT = 1, 2
 KVFX_MAX_LAYERS = 128
 KVFX_MAX_PREFILL_SEQS = 32
+KVFX_NO_SLOT = 2**64 - 1
 
 
 class KvfxCache(ctypes.Structure):
@@ -55,6 +56,21 @@ class KvfxCache(ctypes.Structure):
     ]
 
 
+class KvfxRotary(ctypes.Structure):
+    """Mirror of ``kvfx_rotary`` (include/kvfx.h)."""
+
+    _fields_ = [
+        ("cos_sin", vp),
+        ("max_positions", u64),
+        ("rotary_dim", u32),
+        ("interleaved", u32),
+        ("q_weight", vp),
+        ("k_weight", vp),
+        ("eps", ctypes.c_float),
+        ("reserved", u32),
+    ]
+
+
 def _load():
     L = ctypes.CDLL(str(_LIB_PATH))
     C = ctypes.POINTER(KvfxCache)
@@ -64,6 +80,10 @@ def _load():
     L.kvfx_copy_page.argtypes = [C, u64, u64, vp]
     L.kvfx_write_layers.argtypes = [C, u32, vp, vp, u64, vp, u64, vp]
     L.kvfx_gather_layers.argtypes = [C, u32, vp, vp, u64, u64, vp, vp, u64, vp]
+    L.kvfx_copy_pages.argtypes = [C, u32, vp, vp, u64, vp]
+    L.kvfx_copy_slots.argtypes = [C, u32, vp, vp, u64, vp]
+    L.kvfx_rotary_table.argtypes = [vp, u64, u32, ctypes.c_double, ctypes.c_double, ctypes.c_int, vp]
+    L.kvfx_write_rotated.argtypes = [C, ctypes.POINTER(KvfxRotary), vp, vp, vp, u64, u64, u64, u32, vp, vp, u64, vp, vp]
     L.kvfx_decode_workspace_bytes.argtypes = [C, u64, u32, u64, u32]
     L.kvfx_decode_workspace_bytes.restype = u64
     L.kvfx_decode_pages_per_split.argtypes = [C, u64, u32, u64, u64]
@@ -88,7 +108,8 @@ lib = _load()
 
 #: Every symbol include/kvfx.h declares (checked by the tests).
 KVFX_SYMBOLS = (
-    "kvfx_write", "kvfx_gather", "kvfx_gather_batch", "kvfx_write_layers", "kvfx_gather_layers", "kvfx_copy_page", "kvfx_decode_workspace_bytes",
+    "kvfx_write", "kvfx_gather", "kvfx_gather_batch", "kvfx_write_layers", "kvfx_gather_layers", "kvfx_copy_page", "kvfx_copy_pages",
+    "kvfx_copy_slots", "kvfx_rotary_table", "kvfx_write_rotated", "kvfx_decode_workspace_bytes",
     "kvfx_decode_pages_per_split", "kvfx_decode", "kvfx_decode_append", "kvfx_decode_noalloc", "kvfx_attention_workspace_bytes",
     "kvfx_attention", "kvfx_attention_batch",
     "kvfx_last_error", "kvfx_device_status", "kvfx_selftest_wait_timeout", "kvfx_version",

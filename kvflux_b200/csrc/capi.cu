@@ -320,6 +320,109 @@ int kvfx_copy_page(const kvfx_cache* cache, uint64_t src_block, uint64_t dst_blo
     return e == cudaSuccess ? KVFX_OK : cuda_fail("page copy launch", e);
 }
 
+namespace {
+
+int check_copy(const kvfx_cache* caches, uint32_t num_layers, const uint64_t* src, const uint64_t* dst, uint64_t n,
+               kvfx::CacheView* views) {
+    if (int rc = make_layer_views(caches, num_layers, views); rc != KVFX_OK) return rc;
+    if (num_layers == 0 || n == 0) return KVFX_OK;
+    if (src == nullptr || dst == nullptr) return fail(KVFX_EINVAL, "source and destination ids must be non-null");
+    if (n > views[0].slot_count) return fail(KVFX_EINVAL, "more copies than the cache has destinations");
+    // The kernels index one page, or 16 tokens of every head, in 32 bits.
+    if (views[0].page_bytes > (1ull << 30) || views[0].row_bytes > (1ull << 26) / views[0].heads) {
+        return fail(KVFX_EINVAL, "pages above 1 GiB, or tokens above 64 MiB, are not supported");
+    }
+    return KVFX_OK;
+}
+
+}  // namespace
+
+int kvfx_copy_pages(const kvfx_cache* caches, uint32_t num_layers, const uint64_t* src_pages,
+                    const uint64_t* dst_pages, uint64_t num_pages, void* stream) {
+    kvfx::CacheView views[KVFX_MAX_LAYERS];
+    if (int rc = check_copy(caches, num_layers, src_pages, dst_pages, num_pages, views); rc != KVFX_OK) return rc;
+    if (num_layers == 0 || num_pages == 0) return KVFX_OK;
+    DeviceScope scope(views[0].device);
+    if (scope.error() != cudaSuccess) return cuda_fail("select device", scope.error());
+    const cudaError_t e = kvfx::launch_copy_pages(views, num_layers, src_pages, dst_pages, num_pages,
+                                                  status_word(views[0].device), static_cast<cudaStream_t>(stream));
+    return e == cudaSuccess ? KVFX_OK : cuda_fail("page copies launch", e);
+}
+
+int kvfx_copy_slots(const kvfx_cache* caches, uint32_t num_layers, const uint64_t* src_slots,
+                    const uint64_t* dst_slots, uint64_t num_slots, void* stream) {
+    kvfx::CacheView views[KVFX_MAX_LAYERS];
+    if (int rc = check_copy(caches, num_layers, src_slots, dst_slots, num_slots, views); rc != KVFX_OK) return rc;
+    if (num_layers == 0 || num_slots == 0) return KVFX_OK;
+    DeviceScope scope(views[0].device);
+    if (scope.error() != cudaSuccess) return cuda_fail("select device", scope.error());
+    const cudaError_t e = kvfx::launch_copy_slots(views, num_layers, src_slots, dst_slots, num_slots,
+                                                  status_word(views[0].device), static_cast<cudaStream_t>(stream));
+    return e == cudaSuccess ? KVFX_OK : cuda_fail("slot copies launch", e);
+}
+
+int kvfx_rotary_table(float* cos_sin, uint64_t max_positions, uint32_t rotary_dim, double base,
+                      double position_scale, int device, void* stream) {
+    if (cos_sin == nullptr) return fail(KVFX_EINVAL, "cos_sin must be non-null");
+    if (max_positions == 0 || rotary_dim == 0 || rotary_dim % 2 != 0) {
+        return fail(KVFX_EINVAL, "max_positions must be positive, rotary_dim positive and even");
+    }
+    if (!(base > 0.0) || !std::isfinite(base) || !std::isfinite(position_scale)) {
+        return fail(KVFX_EINVAL, "base must be positive and finite, position_scale finite");
+    }
+    if (device < 0) return fail(KVFX_EINVAL, "device ordinal must be non-negative");
+    uint64_t elems = 0, bytes = 0;
+    if (!mul_ok(max_positions, rotary_dim, &elems) || !mul_ok(elems, sizeof(float), &bytes)) {
+        return fail(KVFX_EOVERFLOW, "rotary table size overflows");
+    }
+    DeviceScope scope(device);
+    if (scope.error() != cudaSuccess) return cuda_fail("select device", scope.error());
+    const cudaError_t e = kvfx::launch_rotary_table(cos_sin, max_positions, rotary_dim, base, position_scale,
+                                                    static_cast<cudaStream_t>(stream));
+    return e == cudaSuccess ? KVFX_OK : cuda_fail("rotary table launch", e);
+}
+
+int kvfx_write_rotated(const kvfx_cache* cache, const kvfx_rotary* rotary, const void* q, const void* k,
+                       const void* v, uint64_t q_stride, uint64_t k_stride, uint64_t v_stride, uint32_t q_heads,
+                       const uint64_t* positions, const uint64_t* slots, uint64_t num_tokens, float* q_out,
+                       void* stream) {
+    kvfx::CacheView c;
+    if (int rc = make_view(cache, &c); rc != KVFX_OK) return rc;
+    if (rotary == nullptr) return fail(KVFX_EINVAL, "rotary descriptor is null");
+    if (rotary->cos_sin == nullptr || rotary->max_positions == 0) return fail(KVFX_EINVAL, "rotary table is empty");
+    if (rotary->rotary_dim == 0 || rotary->rotary_dim % 2 != 0 || rotary->rotary_dim > c.hd) {
+        return fail(KVFX_EINVAL, "rotary_dim must be even, positive and at most head_size");
+    }
+    if (rotary->interleaved > 1) return fail(KVFX_EINVAL, "interleaved must be 0 or 1");
+    if (!(rotary->eps >= 0.f) || !std::isfinite(rotary->eps)) return fail(KVFX_EINVAL, "eps must be finite, not below 0");
+    if (rotary->reserved != 0) return fail(KVFX_EINVAL, "kvfx_rotary.reserved must be 0");
+    if (q_heads > (1u << 30) || c.heads > (1u << 30)) return fail(KVFX_EINVAL, "more than 2^30 heads");
+    if (num_tokens == 0) return KVFX_OK;
+    if (k == nullptr || v == nullptr || positions == nullptr || slots == nullptr ||
+        (q_heads != 0 && (q == nullptr || q_out == nullptr))) {
+        return fail(KVFX_EINVAL, "q, k, v, positions, slots and q_out must be non-null");
+    }
+    uint64_t kv_row = 0, q_row = 0, elems = 0, bytes = 0;
+    if (!mul_ok(c.heads, c.hd, &kv_row) || !mul_ok(q_heads, c.hd, &q_row)) {
+        return fail(KVFX_EOVERFLOW, "token size overflows");
+    }
+    if (k_stride < kv_row || v_stride < kv_row || (q_heads != 0 && q_stride < q_row)) {
+        return fail(KVFX_EINVAL, "a stride is smaller than one token's heads");
+    }
+    for (const uint64_t stride : {q_heads != 0 ? std::max(q_stride, q_row) : uint64_t{0}, k_stride, v_stride}) {
+        if (!mul_ok(num_tokens, stride, &elems) || !mul_ok(elems, sizeof(float), &bytes)) {
+            return fail(KVFX_EOVERFLOW, "rotated write size overflows");
+        }
+    }
+    DeviceScope scope(c.device);
+    if (scope.error() != cudaSuccess) return cuda_fail("select device", scope.error());
+    const kvfx::RotatedArgs a{q_heads != 0 ? q : nullptr, k, v, q_heads != 0 ? q_stride : 0, k_stride, v_stride,
+                              q_heads, positions, slots, num_tokens, q_heads != 0 ? q_out : nullptr};
+    const cudaError_t e = kvfx::launch_write_rotated(c, *rotary, a, status_word(c.device),
+                                                     static_cast<cudaStream_t>(stream));
+    return e == cudaSuccess ? KVFX_OK : cuda_fail("rotated KV write launch", e);
+}
+
 uint32_t kvfx_decode_pages_per_split(const kvfx_cache* cache, uint64_t batch, uint32_t q_heads,
                                      uint64_t max_seq_len, uint64_t total_tokens) {
     kvfx::CacheView c;

@@ -9,10 +9,48 @@
 #include <cuda_runtime.h>
 #include <stdint.h>
 
+#include <utility>
+
 #include "kvfx.h"
 #include "launch.h"
 
 namespace kvfx {
+
+// ------------------------------------------------------------- byte moves ---
+
+// The unsigned type of VB bytes that the byte-moving kernels copy with.
+template <int VB> struct Vec;
+template <> struct Vec<16> { using T = uint4; };
+template <> struct Vec<8> { using T = uint2; };
+template <> struct Vec<4> { using T = uint32_t; };
+template <> struct Vec<2> { using T = uint16_t; };
+template <> struct Vec<1> { using T = uint8_t; };
+
+// Cache bases of the layers of a layer batch (a kernel parameter).
+struct LayerBases {
+    char* k[KVFX_MAX_LAYERS];
+    char* v[KVFX_MAX_LAYERS];
+};
+
+// Launches `kernel` as a programmatic dependent of the stream's previous
+// kernel: its CTAs may be scheduled while that kernel drains (the kernel
+// waits for it with pdl_wait before touching memory). Short write launches
+// that follow one another - a serving loop's steps, a graph of them - then
+// lose the launch gap between them.
+template <typename... KArgs, typename... Args>
+cudaError_t launch_dependent(void (*kernel)(KArgs...), dim3 grid, dim3 block, cudaStream_t s, Args&&... args) {
+    cudaLaunchConfig_t cfg{};
+    cfg.gridDim = grid;
+    cfg.blockDim = block;
+    cfg.dynamicSmemBytes = 0;
+    cfg.stream = s;
+    cudaLaunchAttribute attr[1];
+    attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr[0].val.programmaticStreamSerializationAllowed = 1;
+    cfg.attrs = attr;
+    cfg.numAttrs = 1;
+    return cudaLaunchKernelEx(&cfg, kernel, std::forward<Args>(args)...);
+}
 
 // --------------------------------------------------------------- division ---
 

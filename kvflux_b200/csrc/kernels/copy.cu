@@ -18,13 +18,6 @@
 namespace kvfx {
 namespace {
 
-template <int VB> struct Vec;
-template <> struct Vec<16> { using T = uint4; };
-template <> struct Vec<8> { using T = uint2; };
-template <> struct Vec<4> { using T = uint32_t; };
-template <> struct Vec<2> { using T = uint16_t; };
-template <> struct Vec<1> { using T = uint8_t; };
-
 // ------------------------------------------------------------------ write ---
 // Thread i moves vector c of row (token, head) for both K and V; consecutive
 // threads cover consecutive vectors of a row, so a 256-byte row is one fully
@@ -58,26 +51,6 @@ __global__ void __launch_bounds__(256) write_kernel(
         k_cache[dst] = kv;
         v_cache[dst] = vv;
     }
-}
-
-// Launches `kernel` as a programmatic dependent of the stream's previous
-// kernel: its CTAs may be scheduled while that kernel drains (the kernel
-// waits for it with pdl_wait before touching memory). Short write launches
-// that follow one another - a serving loop's steps, a graph of them - then
-// lose the launch gap between them.
-template <typename... KArgs, typename... Args>
-cudaError_t launch_dependent(void (*kernel)(KArgs...), dim3 grid, dim3 block, cudaStream_t s, Args&&... args) {
-    cudaLaunchConfig_t cfg{};
-    cfg.gridDim = grid;
-    cfg.blockDim = block;
-    cfg.dynamicSmemBytes = 0;
-    cfg.stream = s;
-    cudaLaunchAttribute attr[1];
-    attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
-    attr[0].val.programmaticStreamSerializationAllowed = 1;
-    cfg.attrs = attr;
-    cfg.numAttrs = 1;
-    return cudaLaunchKernelEx(&cfg, kernel, std::forward<Args>(args)...);
 }
 
 template <int VB>
@@ -300,11 +273,8 @@ __global__ void __launch_bounds__(kGatherDirectThreads) gather_direct_kernel(
 // ---------------------------------------------------------- layer batches ---
 // One launch over the caches of num_layers layers that share a page pool
 // (one PagedKVStorage per layer): blockIdx.y (write) or blockIdx.z (gather)
-// selects the layer, whose cache bases come from the kernel parameters.
-struct LayerBases {
-    char* k[KVFX_MAX_LAYERS];
-    char* v[KVFX_MAX_LAYERS];
-};
+// selects the layer, whose cache bases (LayerBases) come from the kernel
+// parameters.
 
 // Vectors of K and of V in flight per thread before its stores. Two (small
 // CTAs, 38 registers, 6 CTAs per SM) measured faster than four or eight at

@@ -42,6 +42,29 @@ cudaError_t launch_write_layers(const CacheView* layers, uint32_t num_layers, co
                                 const void* v_new, uint64_t layer_stride, const uint64_t* slots, uint64_t n,
                                 unsigned* status, cudaStream_t s);
 
+// Page and slot copies inside the caches of a layer batch (layers of one shape).
+cudaError_t launch_copy_pages(const CacheView* layers, uint32_t num_layers, const uint64_t* src, const uint64_t* dst,
+                              uint64_t n, unsigned* status, cudaStream_t s);
+cudaError_t launch_copy_slots(const CacheView* layers, uint32_t num_layers, const uint64_t* src, const uint64_t* dst,
+                              uint64_t n, unsigned* status, cudaStream_t s);
+
+// Norm, rotation and write of new tokens (strides in elements).
+struct RotatedArgs {
+    const void* q;
+    const void* k;
+    const void* v;
+    uint64_t q_stride, k_stride, v_stride;
+    uint32_t q_heads;
+    const uint64_t* positions;
+    const uint64_t* slots;
+    uint64_t tokens;
+    float* q_out;
+};
+cudaError_t launch_write_rotated(const CacheView& c, const kvfx_rotary& rotary, const RotatedArgs& a,
+                                 unsigned* status, cudaStream_t s);
+cudaError_t launch_rotary_table(float* cos_sin, uint64_t max_positions, uint32_t rotary_dim, double base,
+                                double position_scale, cudaStream_t s);
+
 // Gather of `batch` sequences. If `per_seq_out` is false, k_out/v_out point to
 // a single sequence's outputs (batch must be 1) and `single_blocks`/`single_len`
 // describe it; otherwise k_out/v_out are device arrays of device pointers and
