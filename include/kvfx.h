@@ -49,6 +49,9 @@ extern "C" {
 /* Most sequences one kvfx_attention_batch call takes. */
 #define KVFX_MAX_PREFILL_SEQS 32u
 
+/* Most groups one kvfx_decode_shared call takes. */
+#define KVFX_MAX_PREFIX_GROUPS 128u
+
 /* Slot of a padding token (kvfx_write_rotated): nothing is written for it. */
 #define KVFX_NO_SLOT UINT64_MAX
 
@@ -236,6 +239,42 @@ int kvfx_decode(const kvfx_cache* cache, const float* q, float* o,
                 uint64_t max_blocks_per_seq, uint32_t q_heads, uint64_t max_seq_len,
                 uint32_t pages_per_split, void* workspace, uint64_t workspace_bytes,
                 void* stream);
+
+/*
+ * Batch decode over groups of rows that share a prefix: the attention of
+ * kvfx_decode, with each group's shared pages read once for all of its rows
+ * instead of once per row. Group g is the next groups[g].rows rows of the
+ * batch, whose first groups[g].prefix_tokens positions (whole pages) are the
+ * same pages: those of the group's first row, whose table entries are read
+ * for them; every row's table still holds all of its pages. The batch is the
+ * groups' rows in order (at most 65535), num_groups at most
+ * KVFX_MAX_PREFIX_GROUPS, prefix_tokens a multiple of block_size, at most
+ * max_seq_len, and 0 where rows share nothing. groups is a host array, read
+ * before the call returns.
+ *   seq_lens  : device uint64[batch], each 0 or in [prefix_tokens of its
+ *               group, max_seq_len]; a row of length 0 is padding: its output
+ *               stays as it was. A row outside its bounds is refused the same
+ *               way and sets KVFX_FLAG_BAD_INDEX.
+ *   workspace : device scratch of kvfx_decode_shared_workspace_bytes(...)
+ *               bytes, 16-byte aligned; nothing is kept in it from call to
+ *               call. Calls that share one must not overlap on the GPU.
+ * The other arguments as for kvfx_decode. 16-bit caches with head_size 64 or
+ * 128, block_size 16 and 16-byte aligned q and o read the prefix on the tensor cores (at
+ * the FP32-class accuracy of the other attention entry points); other shapes
+ * run row by row, each reading its whole table row. No counterpart in the
+ * reference, whose batch attention re-reads shared pages for every row
+ * (src/v2/paged_attention.cu:248-313).
+ */
+typedef struct kvfx_prefix_group {
+    uint64_t rows;           /* >= 1 */
+    uint64_t prefix_tokens;
+} kvfx_prefix_group;
+uint64_t kvfx_decode_shared_workspace_bytes(const kvfx_cache* cache, const kvfx_prefix_group* groups,
+                                            uint32_t num_groups, uint32_t q_heads, uint64_t max_seq_len);
+int kvfx_decode_shared(const kvfx_cache* cache, const float* q, float* o, const uint64_t* block_table,
+                       const uint64_t* seq_lens, const kvfx_prefix_group* groups, uint32_t num_groups,
+                       uint64_t max_blocks_per_seq, uint32_t q_heads, uint64_t max_seq_len,
+                       void* workspace, uint64_t workspace_bytes, void* stream);
 
 /*
  * One batch decode step fused with its paged KV write. Row b's new token is

@@ -37,6 +37,7 @@ KVFX_F16, KVFX_BF16, KVFX_F32 = 0, 1, 2
 KVFX_FLAG_BAD_INDEX, KVFX_FLAG_TIMEOUT = 1, 2
 KVFX_MAX_LAYERS = 128
 KVFX_MAX_PREFILL_SEQS = 32
+KVFX_MAX_PREFIX_GROUPS = 128
 KVFX_NO_SLOT = 2**64 - 1
 
 
@@ -54,6 +55,12 @@ class KvfxCache(ctypes.Structure):
         ("device", ctypes.c_int32),
         ("reserved", u32),
     ]
+
+
+class KvfxPrefixGroup(ctypes.Structure):
+    """Mirror of ``kvfx_prefix_group`` (include/kvfx.h)."""
+
+    _fields_ = [("rows", u64), ("prefix_tokens", u64)]
 
 
 class KvfxRotary(ctypes.Structure):
@@ -91,6 +98,10 @@ def _load():
     L.kvfx_decode.argtypes = [C, vp, vp, vp, vp, u64, u64, u32, u64, u32, vp, u64, vp]
     L.kvfx_decode_append.argtypes = [C, vp, vp, vp, vp, vp, vp, vp, u64, u64, u32, u64, u32, vp, u64, vp]
     L.kvfx_decode_noalloc.argtypes = [C, vp, vp, vp, vp, u64, u64, u32, u64, vp]
+    G = ctypes.POINTER(KvfxPrefixGroup)
+    L.kvfx_decode_shared_workspace_bytes.argtypes = [C, G, u32, u32, u64]
+    L.kvfx_decode_shared_workspace_bytes.restype = u64
+    L.kvfx_decode_shared.argtypes = [C, vp, vp, vp, vp, G, u32, u64, u32, u64, vp, u64, vp]
     L.kvfx_attention_workspace_bytes.argtypes = [C, u64, u64, u32]
     L.kvfx_attention_workspace_bytes.restype = u64
     L.kvfx_attention.argtypes = [C, vp, vp, vp, u64, u64, u32, vp, u64, vp]
@@ -110,7 +121,8 @@ lib = _load()
 KVFX_SYMBOLS = (
     "kvfx_write", "kvfx_gather", "kvfx_gather_batch", "kvfx_write_layers", "kvfx_gather_layers", "kvfx_copy_page", "kvfx_copy_pages",
     "kvfx_copy_slots", "kvfx_rotary_table", "kvfx_write_rotated", "kvfx_decode_workspace_bytes",
-    "kvfx_decode_pages_per_split", "kvfx_decode", "kvfx_decode_append", "kvfx_decode_noalloc", "kvfx_attention_workspace_bytes",
+    "kvfx_decode_pages_per_split", "kvfx_decode", "kvfx_decode_append", "kvfx_decode_noalloc",
+    "kvfx_decode_shared_workspace_bytes", "kvfx_decode_shared", "kvfx_attention_workspace_bytes",
     "kvfx_attention", "kvfx_attention_batch",
     "kvfx_last_error", "kvfx_device_status", "kvfx_selftest_wait_timeout", "kvfx_version",
 )

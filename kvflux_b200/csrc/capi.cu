@@ -512,6 +512,78 @@ int kvfx_decode_append(const kvfx_cache* cache, const void* k_new, const void* v
     return e == cudaSuccess ? KVFX_OK : cuda_fail("batch decode append launch", e);
 }
 
+namespace {
+
+// The groups' rows and prefixes against the batch's bounds; *batch = all rows.
+int check_groups(const kvfx::CacheView& c, const kvfx_prefix_group* groups, uint32_t num_groups, uint32_t q_heads,
+                 uint64_t max_seq_len, uint64_t* batch) {
+    *batch = 0;
+    if (q_heads == 0 || q_heads % c.heads != 0) {
+        return fail(KVFX_EINVAL, "q_heads must be a positive multiple of num_kv_heads");
+    }
+    if (num_groups > KVFX_MAX_PREFIX_GROUPS) return fail(KVFX_EINVAL, "more groups than KVFX_MAX_PREFIX_GROUPS");
+    if (num_groups == 0) return KVFX_OK;
+    if (groups == nullptr) return fail(KVFX_EINVAL, "groups must be non-null");
+    if (max_seq_len == 0) return fail(KVFX_EINVAL, "max_seq_len must be positive");
+    for (uint32_t g = 0; g < num_groups; ++g) {
+        if (groups[g].rows == 0) return fail(KVFX_EINVAL, "a prefix group has no rows");
+        if (groups[g].rows > 65535 - *batch) return fail(KVFX_EINVAL, "batch above 65535 sequences per launch");
+        if (groups[g].prefix_tokens % c.bs != 0) {
+            return fail(KVFX_EINVAL, "prefix_tokens must be a multiple of block_size");
+        }
+        if (groups[g].prefix_tokens > max_seq_len) return fail(KVFX_EINVAL, "prefix_tokens above max_seq_len");
+        *batch += groups[g].rows;
+    }
+    return KVFX_OK;
+}
+
+}  // namespace
+
+uint64_t kvfx_decode_shared_workspace_bytes(const kvfx_cache* cache, const kvfx_prefix_group* groups,
+                                            uint32_t num_groups, uint32_t q_heads, uint64_t max_seq_len) {
+    kvfx::CacheView c;
+    uint64_t batch = 0;
+    if (make_view(cache, &c) != KVFX_OK || check_groups(c, groups, num_groups, q_heads, max_seq_len, &batch) != KVFX_OK ||
+        batch == 0) {
+        return 0;
+    }
+    return kvfx::shared_workspace_bytes(c, groups, num_groups, q_heads, max_seq_len);
+}
+
+int kvfx_decode_shared(const kvfx_cache* cache, const float* q, float* o, const uint64_t* block_table,
+                       const uint64_t* seq_lens, const kvfx_prefix_group* groups, uint32_t num_groups,
+                       uint64_t max_blocks_per_seq, uint32_t q_heads, uint64_t max_seq_len, void* workspace,
+                       uint64_t workspace_bytes, void* stream) {
+    kvfx::CacheView c;
+    if (int rc = make_view(cache, &c); rc != KVFX_OK) return rc;
+    uint64_t batch = 0;
+    if (int rc = check_groups(c, groups, num_groups, q_heads, max_seq_len, &batch); rc != KVFX_OK) return rc;
+    if (batch == 0) return KVFX_OK;
+    if (q == nullptr || o == nullptr || block_table == nullptr || seq_lens == nullptr) {
+        return fail(KVFX_EINVAL, "q, o, block_table and seq_lens must be non-null");
+    }
+    if (max_blocks_per_seq < kvfx::ceil_div(max_seq_len, c.bs)) {
+        return fail(KVFX_EINVAL, "max_blocks_per_seq is smaller than max_seq_len needs");
+    }
+    uint64_t elems = 0, tmp = 0;
+    if (!mul_ok(batch, q_heads, &tmp) || !mul_ok(tmp, c.hd, &elems) || !mul_ok(batch, max_blocks_per_seq, &tmp)) {
+        return fail(KVFX_EOVERFLOW, "query or block table size overflows");
+    }
+    const uint64_t need = kvfx::shared_workspace_bytes(c, groups, num_groups, q_heads, max_seq_len);
+    if (need != 0 && (workspace == nullptr || workspace_bytes < need)) {
+        return fail(KVFX_ENOSPACE, "workspace is smaller than kvfx_decode_shared_workspace_bytes()");
+    }
+    if (need != 0 && reinterpret_cast<uintptr_t>(workspace) % 16 != 0) {
+        return fail(KVFX_EINVAL, "workspace must be 16-byte aligned");
+    }
+    DeviceScope scope(c.device);
+    if (scope.error() != cudaSuccess) return cuda_fail("select device", scope.error());
+    const kvfx::SharedArgs a{q, o, block_table, seq_lens, max_blocks_per_seq, max_seq_len, q_heads,
+                             groups, num_groups, workspace};
+    const cudaError_t e = kvfx::launch_decode_shared(c, a, status_word(c.device), static_cast<cudaStream_t>(stream));
+    return e == cudaSuccess ? KVFX_OK : cuda_fail("shared-prefix decode launch", e);
+}
+
 uint64_t kvfx_attention_workspace_bytes(const kvfx_cache* cache, uint64_t query_tokens, uint64_t kv_tokens,
                                         uint32_t q_heads) {
     kvfx::CacheView c;

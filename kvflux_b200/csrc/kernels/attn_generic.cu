@@ -35,6 +35,7 @@ struct GenericParams {
     uint64_t num_blocks;
     uint32_t q_heads, kv_heads, bs, hd;
     float qscale;
+    bool skip_empty;
     unsigned* status;
 };
 
@@ -53,6 +54,7 @@ __global__ void __launch_bounds__(kWarps * 32) attn_generic_kernel(const Generic
     if (p.lens != nullptr) {
         visible = p.lens[u];
         brow = p.blocks + u * p.row_stride;
+        if (visible == 0 && p.skip_empty) return;
         if (visible == 0 || visible > p.row_stride * p.bs) {  // outside the table row: refuse
             if (lane == 0) raise_flag(p.status, KVFX_FLAG_BAD_INDEX);
             return;
@@ -171,6 +173,7 @@ cudaError_t launch_attention_generic(const CacheView& c, const GenericAttnArgs& 
     p.bs = c.bs;
     p.hd = c.hd;
     p.qscale = static_cast<float>(1.4426950408889634 / std::sqrt(static_cast<double>(c.hd)));
+    p.skip_empty = a.skip_empty;
     p.status = status;
     switch (c.dtype) {
     case KVFX_F16: return launch_t<__half>(p, s);

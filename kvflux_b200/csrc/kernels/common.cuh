@@ -356,4 +356,17 @@ __device__ __forceinline__ void split2(float x0, float x1, uint32_t& hi, uint32_
     lo = Elem<T>::pack(x0 - Elem<T>::to_f32(h0), x1 - Elem<T>::to_f32(h1));
 }
 
+// The two 16-bit values of a packed pair, widened to float (low half first).
+template <typename T>
+__device__ __forceinline__ uint64_t widen2(uint32_t h);
+template <>
+__device__ __forceinline__ uint64_t widen2<__nv_bfloat16>(uint32_t h) {
+    return f2_pack(__uint_as_float(h << 16), __uint_as_float(h & 0xFFFF0000u));
+}
+template <>
+__device__ __forceinline__ uint64_t widen2<__half>(uint32_t h) {
+    const __half2 x = *reinterpret_cast<const __half2*>(&h);
+    return f2_pack(__low2float(x), __high2float(x));
+}
+
 }  // namespace kvfx

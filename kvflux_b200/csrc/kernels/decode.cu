@@ -33,9 +33,16 @@
 // new K/V row of its head into the cache, replaces the row in its shared-
 // memory tiles, and takes the page from the token's slot, so the launch needs
 // neither a separate write kernel nor a host update of the table.
+//
+// Tail mode (kvfx_decode_shared): the same kernel over the pages behind each
+// row's shared prefix. A row's pages start at its group's prefix, every split
+// leaves its (max, sum, O) in the workspace, and the merge kernel of
+// shared.cu joins them with the prefix's. Query groups above 8 heads take one
+// CTA per 8 heads (blockIdx.y = KV head * chunks + chunk).
 #include <algorithm>
 #include <atomic>
 #include <cmath>
+#include <type_traits>
 
 #include "common.cuh"
 #include "launch.h"
@@ -92,11 +99,22 @@ __device__ __forceinline__ uint32_t swz(int t, int c) {
     return static_cast<uint32_t>((c >> 3) * 2048 + t * 128 + (((c & 7) ^ (t & 7)) << 4));
 }
 
-template <int HD, typename T>
+// The kernel's Tail parameter: a plain decode has none.
+struct NoTail {};
+struct PrefixTail {
+    PrefixGroups groups;
+    uint64_t max_len;     // host bound of the lengths
+    uint32_t q_group;     // query heads per KV head
+    uint32_t chunks;      // CTAs per KV head: ceil(q_group / 8)
+    uint32_t after_prefix;  // launched as a dependent of the prefix kernel
+};
+
+template <int HD, typename T, typename Tail>
 __global__ void __launch_bounds__(kWarps * 32, 3)
 decode_mma_kernel(const __grid_constant__ DecodeParams p, const __grid_constant__ CUtensorMap kmap,
-                  const __grid_constant__ CUtensorMap vmap) {
+                  const __grid_constant__ CUtensorMap vmap, const __grid_constant__ Tail tail) {
     using S = Shape<HD>;
+    constexpr bool kTail = std::is_same<Tail, PrefixTail>::value;
     extern __shared__ unsigned char smem_raw[];
     __shared__ uint64_t bars[kWarps][kStages];
     __shared__ float s_m[kWarps][8], s_l[kWarps][8];
@@ -106,24 +124,56 @@ decode_mma_kernel(const __grid_constant__ DecodeParams p, const __grid_constant_
     unsigned char* smem = reinterpret_cast<unsigned char*>(
         (reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
-    const uint32_t split = blockIdx.x, kh = blockIdx.y;
+    const uint32_t split = blockIdx.x;
     const uint64_t r = blockIdx.z;
+    // KV head, its first query head and how many this CTA takes (<= 8).
+    uint32_t kh = blockIdx.y, qh0, G;
+    if constexpr (kTail) {
+        kh = blockIdx.y / tail.chunks;
+        const uint32_t chunk = blockIdx.y - kh * tail.chunks;
+        qh0 = kh * tail.q_group + chunk * 8;
+        G = min(8u, tail.q_group - chunk * 8);
+    } else {
+        qh0 = kh * p.group;
+        G = p.group;
+    }
 
     // Launched as a programmatic dependent: the stream's next kernel may be
     // scheduled as soon as every CTA of this one has started (so its CTAs
     // take the SMs this launch's last wave leaves), and this one reads
     // nothing before the kernel ahead of it has completed.
     pdl_allow_next();
-    pdl_wait();
+    if constexpr (kTail) {
+        // The prefix kernel lets this one start once its own wait is over, so
+        // everything before it is complete; it writes nothing that is read
+        // here. Every exit below waits for it all the same, so that the end
+        // of this launch means the end of that one.
+        if (tail.after_prefix == 0) pdl_wait();
+    } else {
+        pdl_wait();
+    }
     const uint64_t len = p.lens != nullptr ? p.lens[r] : p.single_len;
     const uint64_t npages = ceil_div(len, 16);
-    const uint32_t nsplits = static_cast<uint32_t>(ceil_div(npages, p.pages_per_split));
-    if (len == 0 || split >= nsplits) return;
-    if (nsplits > p.max_splits || npages > p.max_blocks) {  // length beyond the host's bounds: refuse
-        if (tid == 0) raise_flag(p.status, KVFX_FLAG_BAD_INDEX);
+    uint64_t first = 0;  // the row's first page here
+    if constexpr (kTail) {
+        first = tail.groups.pages[tail.groups.of_row(static_cast<uint32_t>(r))];
+        // Rows outside the bounds are refused (and flagged) by the merge kernel.
+        if (len > tail.max_len || npages <= first) {
+            pdl_wait();
+            return;
+        }
+    }
+    const uint32_t nsplits = static_cast<uint32_t>(ceil_div(npages - first, p.pages_per_split));
+    if (len == 0 || split >= nsplits) {
+        if constexpr (kTail) pdl_wait();
         return;
     }
-    const uint64_t pbeg = static_cast<uint64_t>(split) * p.pages_per_split;
+    if (nsplits > p.max_splits || npages > p.max_blocks) {  // length beyond the host's bounds: refuse
+        if (tid == 0) raise_flag(p.status, KVFX_FLAG_BAD_INDEX);
+        if constexpr (kTail) pdl_wait();
+        return;
+    }
+    const uint64_t pbeg = first + static_cast<uint64_t>(split) * p.pages_per_split;
     const uint64_t pend = umin64(npages, pbeg + p.pages_per_split);
     const uint64_t* row = p.table + r * p.max_blocks;
     const uint32_t n_my =
@@ -218,11 +268,13 @@ decode_mma_kernel(const __grid_constant__ DecodeParams p, const __grid_constant_
 
     // Q fragments (A operand): rows g = hi(Q[g]), rows g+8 = lo(Q[g]).
     const int g = lane >> 2, tig = lane & 3;
-    const bool live = static_cast<uint32_t>(g) < p.group;
+    const bool live = static_cast<uint32_t>(g) < G;
     uint32_t qa[S::kKSteps][4];
     {
-        const uint64_t qh = static_cast<uint64_t>(kh) * p.group + (live ? g : 0);
-        const float* qrow = p.q + (r * p.kv_heads * p.group + qh) * HD;
+        const uint64_t qh = static_cast<uint64_t>(qh0) + (live ? g : 0);
+        uint32_t q_heads = p.kv_heads * p.group;
+        if constexpr (kTail) q_heads = p.kv_heads * tail.q_group;
+        const float* qrow = p.q + (r * q_heads + qh) * HD;
 #pragma unroll
         for (int kk = 0; kk < S::kKSteps; ++kk) {
             const int c0 = 16 * kk + 2 * tig;
@@ -351,7 +403,7 @@ decode_mma_kernel(const __grid_constant__ DecodeParams p, const __grid_constant_
     // A load never arrived (status already flagged): no O from this CTA; a
     // split still counts itself with an empty partial (below).
     const bool failed = s_flag != 0;
-    if (failed && nsplits == 1) return;
+    if (!kTail && failed && nsplits == 1) return;
 
     float* mo = reinterpret_cast<float*>(smem);  // [kWarps][8][HD]
     if (!failed) {
@@ -372,7 +424,6 @@ decode_mma_kernel(const __grid_constant__ DecodeParams p, const __grid_constant_
         }
     }
     __syncthreads();
-    const uint32_t G = p.group;
     if (!failed && tid < static_cast<int>(G)) {
         float M = -INFINITY;
         for (int w = 0; w < kWarps; ++w) M = fmaxf(M, s_m[w][tid]);
@@ -388,8 +439,8 @@ decode_mma_kernel(const __grid_constant__ DecodeParams p, const __grid_constant_
     }
     __syncthreads();
 
-    const uint64_t pair = r * p.kv_heads + kh;
-    if (nsplits == 1) {
+    const uint64_t pair = r * (kTail ? gridDim.y : p.kv_heads) + (kTail ? blockIdx.y : kh);
+    if (!kTail && nsplits == 1) {
         for (uint32_t idx = tid; idx < G * HD; idx += kWarps * 32) {
             const uint32_t gg = idx / HD, d = idx - gg * HD;
             float acc = 0.f;
@@ -413,6 +464,10 @@ decode_mma_kernel(const __grid_constant__ DecodeParams p, const __grid_constant_
     if (tid < static_cast<int>(G)) {
         part[tid * (HD + 2) + HD] = failed ? -INFINITY : s_m[0][tid];
         part[tid * (HD + 2) + HD + 1] = failed ? 0.f : s_l[0][tid];
+    }
+    if constexpr (kTail) {
+        pdl_wait();
+        return;
     }
     __threadfence();
     __syncthreads();
@@ -499,7 +554,7 @@ cudaError_t launch_fast(const CacheView& c, const DecodeArgs& a, const CacheMaps
     static std::atomic<int> attr_done[64];  // zero-initialised (static storage)
     if (c.device < 0 || c.device >= 64 || !attr_done[c.device].load(std::memory_order_acquire)) {
         // Idempotent: threads that race here all set the same attribute.
-        cudaError_t e = cudaFuncSetAttribute(decode_mma_kernel<HD, T>,
+        cudaError_t e = cudaFuncSetAttribute(decode_mma_kernel<HD, T, NoTail>,
                                              cudaFuncAttributeMaxDynamicSharedMemorySize, Sh::kSmem);
         if (e != cudaSuccess) return e;
         if (c.device >= 0 && c.device < 64) attr_done[c.device].store(1, std::memory_order_release);
@@ -536,7 +591,46 @@ cudaError_t launch_fast(const CacheView& c, const DecodeArgs& a, const CacheMaps
     attr[0].val.programmaticStreamSerializationAllowed = 1;
     cfg.attrs = attr;
     cfg.numAttrs = 1;
-    return cudaLaunchKernelEx(&cfg, decode_mma_kernel<HD, T>, p, maps->k, maps->v);
+    return cudaLaunchKernelEx(&cfg, decode_mma_kernel<HD, T, NoTail>, p, maps->k, maps->v, NoTail{});
+}
+
+// Tail mode: grid (splits, KV heads x chunks, rows), partials only.
+template <int HD, typename T>
+cudaError_t launch_tail(const CacheView& c, const TailArgs& a, const CacheMaps* maps, unsigned* status,
+                        cudaStream_t s) {
+    using Sh = Shape<HD>;
+    static std::atomic<int> attr_done[64];  // zero-initialised (static storage)
+    if (c.device < 0 || c.device >= 64 || !attr_done[c.device].load(std::memory_order_acquire)) {
+        cudaError_t e = cudaFuncSetAttribute(decode_mma_kernel<HD, T, PrefixTail>,
+                                             cudaFuncAttributeMaxDynamicSharedMemorySize, Sh::kSmem);
+        if (e != cudaSuccess) return e;
+        if (c.device >= 0 && c.device < 64) attr_done[c.device].store(1, std::memory_order_release);
+    }
+    DecodeParams p{};
+    p.q = a.q;
+    p.table = a.table;
+    p.lens = a.lens;
+    p.max_blocks = a.max_blocks;
+    p.num_blocks = c.num_blocks;
+    p.kv_heads = c.heads;
+    p.pages_per_split = a.pages_per_split;
+    p.max_splits = a.max_splits;
+    p.qscale = static_cast<float>(1.4426950408889634 / std::sqrt(static_cast<double>(c.hd)));
+    p.partial = a.partial;
+    p.status = status;
+    const uint32_t q_group = a.q_heads / c.heads, chunks = (q_group + 7) / 8;
+    const PrefixTail tail{*a.groups, a.max_len, q_group, chunks, a.after_prefix ? 1u : 0u};
+    cudaLaunchConfig_t cfg{};
+    cfg.gridDim = dim3(a.max_splits, c.heads * chunks, a.groups->rows());
+    cfg.blockDim = dim3(kWarps * 32);
+    cfg.dynamicSmemBytes = Sh::kSmem;
+    cfg.stream = s;
+    cudaLaunchAttribute attr[1];
+    attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr[0].val.programmaticStreamSerializationAllowed = 1;
+    cfg.attrs = attr;
+    cfg.numAttrs = 1;
+    return cudaLaunchKernelEx(&cfg, decode_mma_kernel<HD, T, PrefixTail>, p, maps->k, maps->v, tail);
 }
 
 uint32_t clamp_pps(const CacheView& c, uint64_t max_len, uint32_t pps) {
@@ -614,6 +708,20 @@ cudaError_t launch_decode(const CacheView& c, const DecodeArgs& a, unsigned* sta
     }
     return c.dtype == KVFX_BF16 ? launch_fast<64, __nv_bfloat16>(c, a, maps, pps, max_splits, status, s)
                                 : launch_fast<64, __half>(c, a, maps, pps, max_splits, status, s);
+}
+
+uint32_t decode_tail_split(const CacheView& c, uint64_t max_pages, uint32_t pps) {
+    return clamp_pps(c, max_pages * c.bs, pps);
+}
+
+cudaError_t launch_decode_tail(const CacheView& c, const TailArgs& a, const CacheMaps& maps, unsigned* status,
+                               cudaStream_t s) {
+    if (c.hd == 128) {
+        return c.dtype == KVFX_BF16 ? launch_tail<128, __nv_bfloat16>(c, a, &maps, status, s)
+                                    : launch_tail<128, __half>(c, a, &maps, status, s);
+    }
+    return c.dtype == KVFX_BF16 ? launch_tail<64, __nv_bfloat16>(c, a, &maps, status, s)
+                                : launch_tail<64, __half>(c, a, &maps, status, s);
 }
 
 cudaError_t launch_decode_with_maps(const CacheView& c, const DecodeArgs& a, const CacheMaps& maps,

@@ -124,6 +124,87 @@ uint32_t decode_pages_per_split(const CacheView& c, uint64_t batch, uint32_t q_h
                                 uint64_t max_len, uint64_t total_tokens);
 cudaError_t launch_decode(const CacheView& c, const DecodeArgs& a, unsigned* status, cudaStream_t s);
 
+// Groups of consecutive batch rows that share their leading pages, as the
+// kernels of kvfx_decode_shared read them (a kernel parameter). Group g holds
+// rows [row_end[g - 1], row_end[g]) and shares pages[g] pages. The prefix
+// kernel's work is `pairs` of one KV head and one tile of 128 query rows
+// (a group's pairs are KV head major), each of ceil(pages / 8) tiles of 128
+// tokens; pair_end and tile_end count them over the groups in order.
+struct PrefixGroups {
+    uint32_t n;
+    uint32_t row_end[KVFX_MAX_PREFIX_GROUPS];
+    uint32_t pages[KVFX_MAX_PREFIX_GROUPS];
+    uint32_t pair_end[KVFX_MAX_PREFIX_GROUPS];
+    uint32_t tile_end[KVFX_MAX_PREFIX_GROUPS];
+
+    __host__ __device__ uint32_t rows() const { return row_end[n - 1]; }
+    __host__ __device__ uint32_t pairs() const { return pair_end[n - 1]; }
+    __host__ __device__ uint32_t tiles() const { return tile_end[n - 1]; }
+    // First group whose count in `end` passes x.
+    __host__ __device__ uint32_t find(const uint32_t* end, uint32_t x) const {
+        uint32_t lo = 0, hi = n - 1;
+        while (lo < hi) {
+            const uint32_t mid = (lo + hi) / 2;
+            if (end[mid] > x) hi = mid;
+            else lo = mid + 1;
+        }
+        return lo;
+    }
+    __host__ __device__ uint32_t of_row(uint32_t row) const { return find(row_end, row); }
+    __host__ __device__ uint32_t of_tile(uint32_t tile) const { return find(tile_end, tile); }
+};
+
+// The rows' own pages behind their groups' prefixes (decode.cu, tail mode):
+// split s of (row, KV head and chunk y) leaves its partial, 8 (hd + 2)
+// floats, at partial[((row * gridDim.y + y) * max_splits + s)].
+struct TailArgs {
+    const float* q;
+    const uint64_t* table;
+    const uint64_t* lens;
+    uint64_t max_blocks, max_len;
+    uint32_t q_heads, pages_per_split, max_splits;
+    const PrefixGroups* groups;
+    float* partial;
+    bool after_prefix;
+};
+// A split size the kernel takes, near `pps`, for rows of at most max_pages.
+uint32_t decode_tail_split(const CacheView& c, uint64_t max_pages, uint32_t pps);
+struct CacheMaps;
+cudaError_t launch_decode_tail(const CacheView& c, const TailArgs& a, const CacheMaps& maps, unsigned* status,
+                               cudaStream_t s);
+
+// The prefix kernel (prefix.cu): `grid` CTAs deal the groups' tiles in equal
+// consecutive runs; a run's part of a pair is a segment, whose running
+// maximum, sum and unnormalised O go to slot (CTA + pair) of part_o
+// [slots][128][hd] and part_ml [slots][128][2].
+struct PrefixArgs {
+    const float* q;
+    const uint64_t* table;
+    uint64_t max_blocks;
+    uint32_t q_heads, grid;
+    const PrefixGroups* groups;
+    float* part_o;
+    float* part_ml;
+};
+cudaError_t launch_prefix_tc(const CacheView& c, const PrefixArgs& a, const CacheMaps& maps, unsigned* status,
+                             cudaStream_t s);
+
+// Shared-prefix batch decode (shared.cu).
+struct SharedArgs {
+    const float* q;
+    float* o;
+    const uint64_t* table;
+    const uint64_t* lens;
+    uint64_t max_blocks, max_len;
+    uint32_t q_heads;
+    const kvfx_prefix_group* groups;
+    uint32_t num_groups;
+    void* workspace;
+};
+uint64_t shared_workspace_bytes(const CacheView& c, const kvfx_prefix_group* groups, uint32_t num_groups,
+                                uint32_t q_heads, uint64_t max_len);
+cudaError_t launch_decode_shared(const CacheView& c, const SharedArgs& a, unsigned* status, cudaStream_t s);
+
 struct AttentionArgs {
     const float* q;
     float* o;
@@ -156,6 +237,7 @@ struct GenericAttnArgs {
     uint64_t units;             // batch size, or query_tokens for a single sequence
     uint64_t kv_tokens;         // single-sequence mode: sequence length
     uint32_t q_heads;
+    bool skip_empty = false;    // batch mode: a length of 0 is a padding row, not an error
 };
 cudaError_t launch_attention_generic(const CacheView& c, const GenericAttnArgs& a,
                                      unsigned* status, cudaStream_t s);

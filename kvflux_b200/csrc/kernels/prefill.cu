@@ -158,19 +158,6 @@ struct TileCursor {
     __device__ __forceinline__ bool last() const { return j + 1 == u.ntiles; }
 };
 
-// The two 16-bit values of a packed pair, widened to float (low half first).
-template <typename T>
-__device__ __forceinline__ uint64_t widen2(uint32_t h);
-template <>
-__device__ __forceinline__ uint64_t widen2<__nv_bfloat16>(uint32_t h) {
-    return f2_pack(__uint_as_float(h << 16), __uint_as_float(h & 0xFFFF0000u));
-}
-template <>
-__device__ __forceinline__ uint64_t widen2<__half>(uint32_t h) {
-    const __half2 x = *reinterpret_cast<const __half2*>(&h);
-    return f2_pack(__low2float(x), __high2float(x));
-}
-
 // Page id of page `lane` of KV tile j of sequence s in lanes 0..7 (one load
 // per lane, all in one memory round trip); 0 in the other lanes.
 __device__ __forceinline__ uint64_t tile_page_id(const PrefillParams& p, uint32_t s, uint32_t j, uint32_t lane) {

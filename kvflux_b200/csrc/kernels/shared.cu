@@ -1,0 +1,246 @@
+// Batch decode over groups of rows that share a prefix (kvfx_decode_shared).
+//
+// A row's softmax over its positions is split at the end of its group's
+// prefix, and each side further; a piece with running maximum m, sum l and
+// unnormalised O joins the others by
+//     M = max m,  L = sum l 2^(m - M),  o = (sum O 2^(m - M)) / L.
+// Three launches, each a programmatic dependent of the one before it:
+//   prefix  (prefix.cu)   the groups' shared pages, once per 128 query rows;
+//   tail    (decode.cu)   each row's own pages behind them;
+//   merge   (below)       the pieces of every (row, query head).
+// The workspace holds the pieces only, so nothing in it outlives a call.
+#include <algorithm>
+#include <cmath>
+
+#include "common.cuh"
+#include "launch.h"
+
+namespace kvfx {
+namespace {
+
+constexpr int kMergeWarps = 4;
+constexpr int kAhead = 4;  // pieces loaded before the first is joined
+
+struct MergeParams {
+    PrefixGroups groups;
+    const uint64_t* lens;
+    float* o;
+    const float* part_o;   // prefix segments: [slot][128][hd], [slot][128][2]
+    const float* part_ml;
+    const float* tail;     // tail splits: [row][heads x chunks][split][8][hd + 2]
+    uint64_t max_len, max_blocks;
+    uint32_t grid;         // CTAs of the prefix launch
+    uint32_t q_heads, kv_heads, q_group, chunks;
+    uint32_t pages_per_split, max_splits;
+    unsigned* status;
+};
+
+// One warp per (row, query head); lane l holds dims 2l, 2l + 1 (and 64 more).
+template <int HD>
+__global__ void __launch_bounds__(kMergeWarps * 32) merge_kernel(const __grid_constant__ MergeParams p) {
+    constexpr int kV = HD / 64;  // float2 per lane
+    pdl_allow_next();
+    pdl_wait();
+    const int lane = threadIdx.x & 31;
+    const uint32_t id = blockIdx.x * kMergeWarps + (threadIdx.x >> 5);
+    const uint32_t row = id / p.q_heads, j = id - row * p.q_heads;
+    if (row >= p.groups.rows()) return;
+    const uint64_t len = __ldg(p.lens + row);
+    if (len == 0) return;  // padding
+    const uint32_t g = p.groups.of_row(row);
+    const uint32_t first = p.groups.pages[g];
+    const uint64_t npages = ceil_div(len, 16);
+    if (len > p.max_len || npages > p.max_blocks || len < static_cast<uint64_t>(first) * 16) {
+        if (lane == 0) raise_flag(p.status, KVFX_FLAG_BAD_INDEX);
+        return;
+    }
+    float M = -INFINITY, L = 0.f;
+    float2 acc[kV];
+#pragma unroll
+    for (int v = 0; v < kV; ++v) acc[v] = make_float2(0.f, 0.f);
+    // Joins up to kAhead pieces; piece i's (m, l) at ml(i) and O at o(i).
+    auto join = [&](uint32_t n, auto&& ml, auto&& o) {
+        float2 s[kAhead], x[kAhead][kV];
+#pragma unroll
+        for (uint32_t i = 0; i < kAhead; ++i) {
+            s[i] = make_float2(-INFINITY, 0.f);
+            if (i < n) {
+                s[i] = __ldcg(reinterpret_cast<const float2*>(ml(i)));
+#pragma unroll
+                for (int v = 0; v < kV; ++v) x[i][v] = __ldcg(reinterpret_cast<const float2*>(o(i)) + lane + 32 * v);
+            }
+        }
+        float m_new = M;
+#pragma unroll
+        for (uint32_t i = 0; i < kAhead; ++i) m_new = fmaxf(m_new, s[i].x);
+        // A piece without any visible score (m = -inf) weighs nothing.
+        const float keep = M == -INFINITY ? 0.f : exp2f(M - m_new);
+        M = m_new;
+        L *= keep;
+#pragma unroll
+        for (int v = 0; v < kV; ++v) acc[v] = make_float2(acc[v].x * keep, acc[v].y * keep);
+#pragma unroll
+        for (uint32_t i = 0; i < kAhead; ++i) {
+            if (i >= n || s[i].x == -INFINITY) continue;
+            const float w = exp2f(s[i].x - M);
+            L = fmaf(s[i].y, w, L);
+#pragma unroll
+            for (int v = 0; v < kV; ++v) {
+                acc[v].x = fmaf(x[i][v].x, w, acc[v].x);
+                acc[v].y = fmaf(x[i][v].y, w, acc[v].y);
+            }
+        }
+    };
+
+    const uint32_t kh = j / p.q_group, gq = j - kh * p.q_group;
+    if (first != 0) {
+        const uint32_t row0 = g == 0 ? 0 : p.groups.row_end[g - 1];
+        const uint32_t tile0 = g == 0 ? 0 : p.groups.tile_end[g - 1], pair0 = g == 0 ? 0 : p.groups.pair_end[g - 1];
+        const uint32_t m = (row - row0) * p.q_group + gq;  // query row in the group's matrix
+        const uint32_t m_tiles = ((p.groups.row_end[g] - row0) * p.q_group + 127) / 128;
+        const uint32_t pair = kh * m_tiles + m / 128;
+        const uint32_t ntiles = (first + 7) / 8;
+        // The CTAs whose runs [tiles c / grid, tiles (c + 1) / grid) meet the pair's tiles.
+        const uint64_t tiles = p.groups.tiles(), t0 = tile0 + static_cast<uint64_t>(pair) * ntiles;
+        auto owner = [&](uint64_t t) { return static_cast<uint32_t>(((t + 1) * p.grid - 1) / tiles); };
+        const uint32_t c0 = owner(t0), n = owner(t0 + ntiles - 1) - c0 + 1;
+        const uint64_t base = (static_cast<uint64_t>(c0 + pair0 + pair)) * 128 + m % 128;
+        for (uint32_t s = 0; s < n; s += kAhead) {
+            join(min(n - s, static_cast<uint32_t>(kAhead)),
+                 [&](uint32_t i) { return p.part_ml + (base + static_cast<uint64_t>(s + i) * 128) * 2; },
+                 [&](uint32_t i) { return p.part_o + (base + static_cast<uint64_t>(s + i) * 128) * HD; });
+        }
+    }
+    const uint32_t n = static_cast<uint32_t>(ceil_div(npages - first, p.pages_per_split));
+    const uint64_t unit = static_cast<uint64_t>(row) * (p.kv_heads * p.chunks) + kh * p.chunks + gq / 8;
+    const float* tail = p.tail + (unit * p.max_splits * 8 + gq % 8) * (HD + 2);
+    for (uint32_t s = 0; s < n; s += kAhead) {
+        join(min(n - s, static_cast<uint32_t>(kAhead)),
+             [&](uint32_t i) { return tail + static_cast<uint64_t>(s + i) * 8 * (HD + 2) + HD; },
+             [&](uint32_t i) { return tail + static_cast<uint64_t>(s + i) * 8 * (HD + 2); });
+    }
+    const float inv = 1.f / L;
+    float2* out = reinterpret_cast<float2*>(p.o + (static_cast<uint64_t>(row) * p.q_heads + j) * HD);
+#pragma unroll
+    for (int v = 0; v < kV; ++v) out[lane + 32 * v] = make_float2(acc[v].x * inv, acc[v].y * inv);
+}
+
+// How a call is cut into pieces, from host-side facts alone (the workspace
+// size and the launches must agree on it).
+struct Plan {
+    PrefixGroups groups;
+    uint32_t grid;             // prefix CTAs (0: nothing shared)
+    uint32_t pages_per_split;  // tail splits
+    uint32_t max_splits;       // 0: no row has pages of its own
+    uint64_t off_ml, off_tail, bytes;
+};
+
+bool fast_shape(const CacheView& c, uint32_t q_heads) {
+    return (c.dtype == KVFX_BF16 || c.dtype == KVFX_F16) && c.bs == 16 && (c.hd == 64 || c.hd == 128) &&
+           c.num_blocks < (1ull << 31) && q_heads <= 65535;
+}
+
+bool make_plan(const CacheView& c, const kvfx_prefix_group* groups, uint32_t n, uint32_t q_heads, uint64_t max_len,
+               Plan* plan) {
+    if (!fast_shape(c, q_heads)) return false;
+    const uint64_t q_group = q_heads / c.heads, max_pages = ceil_div(max_len, 16);
+    if (max_pages >= (1ull << 31)) return false;
+    PrefixGroups& gs = plan->groups;
+    gs.n = n;
+    uint64_t rows = 0, pairs = 0, tiles = 0, tail_pages = 0;
+    for (uint32_t g = 0; g < n; ++g) {
+        const uint64_t pages = groups[g].prefix_tokens / 16;
+        const uint64_t group_pairs = pages != 0 ? c.heads * ceil_div(groups[g].rows * q_group, 128) : 0;
+        rows += groups[g].rows;
+        pairs += group_pairs;
+        tiles += group_pairs * ceil_div(pages, 8);
+        if (pairs >= (1ull << 31) || tiles >= (1ull << 31)) return false;
+        tail_pages = std::max(tail_pages, max_pages - pages);
+        gs.row_end[g] = static_cast<uint32_t>(rows);
+        gs.pages[g] = static_cast<uint32_t>(pages);
+        gs.pair_end[g] = static_cast<uint32_t>(pairs);
+        gs.tile_end[g] = static_cast<uint32_t>(tiles);
+    }
+    plan->grid = static_cast<uint32_t>(umin64(tiles, device_sm_count(c.device)));
+    plan->pages_per_split = 1;
+    plan->max_splits = 0;
+    if (tail_pages != 0) {
+        plan->pages_per_split = decode_tail_split(
+            c, tail_pages, decode_pages_per_split(c, rows, q_heads, tail_pages * 16, 0));
+        plan->max_splits = static_cast<uint32_t>(ceil_div(tail_pages, plan->pages_per_split));
+    }
+    const uint64_t slots = plan->grid != 0 ? plan->grid + pairs : 0;
+    auto align = [](uint64_t b) { return (b + 255) & ~uint64_t(255); };
+    plan->off_ml = align(slots * 128 * c.hd * 4);
+    plan->off_tail = plan->off_ml + align(slots * 128 * 8);
+    plan->bytes = plan->off_tail +
+                  align(rows * c.heads * ceil_div(q_group, 8) * plan->max_splits * 8 * (c.hd + 2) * 4);
+    return true;
+}
+
+template <int HD>
+cudaError_t launch_merge(const MergeParams& p, uint32_t rows, cudaStream_t s) {
+    const uint64_t items = static_cast<uint64_t>(rows) * p.q_heads;
+    return launch_dependent(merge_kernel<HD>, dim3(static_cast<uint32_t>(ceil_div(items, kMergeWarps))),
+                            dim3(kMergeWarps * 32), s, p);
+}
+
+}  // namespace
+
+uint64_t shared_workspace_bytes(const CacheView& c, const kvfx_prefix_group* groups, uint32_t num_groups,
+                                uint32_t q_heads, uint64_t max_len) {
+    Plan plan;
+    return make_plan(c, groups, num_groups, q_heads, max_len, &plan) ? plan.bytes : 0;
+}
+
+cudaError_t launch_decode_shared(const CacheView& c, const SharedArgs& a, unsigned* status, cudaStream_t s) {
+    Plan plan;
+    const bool aligned = ((reinterpret_cast<uintptr_t>(a.q) | reinterpret_cast<uintptr_t>(a.o)) & 15u) == 0;
+    if (!make_plan(c, a.groups, a.num_groups, a.q_heads, a.max_len, &plan) || !aligned) {
+        // Row by row over the whole table.
+        uint64_t rows = 0;
+        for (uint32_t g = 0; g < a.num_groups; ++g) rows += a.groups[g].rows;
+        GenericAttnArgs g{a.q, a.o, a.table, a.max_blocks, a.lens, rows, 0, a.q_heads};
+        g.skip_empty = true;
+        return launch_attention_generic(c, g, status, s);
+    }
+    cudaError_t err = cudaSuccess;
+    const CacheMaps* maps = cache_maps(c, &err);
+    if (maps == nullptr) return err != cudaSuccess ? err : cudaErrorInvalidValue;
+    char* ws = static_cast<char*>(a.workspace);
+    float* part_o = reinterpret_cast<float*>(ws);
+    float* part_ml = reinterpret_cast<float*>(ws + plan.off_ml);
+    float* tail = reinterpret_cast<float*>(ws + plan.off_tail);
+    if (plan.grid != 0) {
+        const PrefixArgs pa{a.q, a.table, a.max_blocks, a.q_heads, plan.grid, &plan.groups, part_o, part_ml};
+        err = launch_prefix_tc(c, pa, *maps, status, s);
+        if (err != cudaSuccess) return err;
+    }
+    if (plan.max_splits != 0) {
+        const TailArgs ta{a.q, a.table, a.lens, a.max_blocks, a.max_len, a.q_heads, plan.pages_per_split,
+                          plan.max_splits, &plan.groups, tail, plan.grid != 0};
+        err = launch_decode_tail(c, ta, *maps, status, s);
+        if (err != cudaSuccess) return err;
+    }
+    MergeParams m;
+    m.groups = plan.groups;
+    m.lens = a.lens;
+    m.o = a.o;
+    m.part_o = part_o;
+    m.part_ml = part_ml;
+    m.tail = tail;
+    m.max_len = a.max_len;
+    m.max_blocks = a.max_blocks;
+    m.grid = plan.grid;
+    m.q_heads = a.q_heads;
+    m.kv_heads = c.heads;
+    m.q_group = a.q_heads / c.heads;
+    m.chunks = (m.q_group + 7) / 8;
+    m.pages_per_split = plan.pages_per_split;
+    m.max_splits = plan.max_splits;
+    m.status = status;
+    const uint32_t rows = plan.groups.rows();
+    return c.hd == 128 ? launch_merge<128>(m, rows, s) : launch_merge<64>(m, rows, s);
+}
+
+}  // namespace kvfx

@@ -54,3 +54,30 @@ def test_rotary_table_refuses_bad_arguments():
                                             (4, 8, float("nan"), 1.0, 0), (4, 8, 1e4, float("inf"), 0), (4, 8, 1e4, 1.0, -1)):
         assert f(1, reach, rot, base, scale, device, None) == kv.KVFX_EINVAL
     assert f(1, 2**61, 8, 1e4, 1.0, 0, None) == kv.KVFX_EOVERFLOW
+
+
+def test_shared_decode_refuses_bad_arguments():
+    c = ctypes.byref(_cache())  # 2 heads, pages of 16
+
+    def f(groups=((2, 32),), n=None, q=16, o=16, table=16, lens=16, width=4, hq=4, max_len=64, ws=None, ws_bytes=0):
+        arr = (kv.KvfxPrefixGroup * max(1, len(groups)))(*groups) if groups is not None else None
+        n = len(groups) if n is None else n
+        return kv.lib.kvfx_decode_shared(c, q, o, table, lens, arr, n, width, hq, max_len, ws, ws_bytes, None)
+
+    assert kv.lib.kvfx_decode_shared(None, 1, 1, 1, 1, None, 0, 4, 4, 64, None, 0, None) == kv.KVFX_EINVAL
+    assert f(groups=(), q=None, o=None, table=None, lens=None) == kv.KVFX_OK
+    for bad in (dict(hq=3), dict(hq=0), dict(groups=None, n=1), dict(groups=((0, 32),)), dict(groups=((2, 33),)), dict(groups=((2, 80),)),
+                dict(groups=((65535, 0), (1, 0))), dict(groups=((2**63, 0), (2**63, 0))), dict(groups=((1, 0),) * 129), dict(q=None), dict(o=None),
+                dict(table=None), dict(lens=None), dict(width=3), dict(max_len=0)):
+        assert f(**bad) == kv.KVFX_EINVAL, bad
+    fast = _cache(num_blocks=1024, num_kv_heads=8, head_size=128)
+    groups = (kv.KvfxPrefixGroup * 2)((8, 512), (3, 0))
+    need = kv.lib.kvfx_decode_shared_workspace_bytes(ctypes.byref(fast), groups, 2, 32, 1024)
+    assert need > 0
+    call = kv.lib.kvfx_decode_shared
+    assert call(ctypes.byref(fast), 16, 16, 16, 16, groups, 2, 64, 32, 1024, 256, need - 1, None) == kv.KVFX_ENOSPACE
+    assert call(ctypes.byref(fast), 16, 16, 16, 16, groups, 2, 64, 32, 1024, None, need, None) == kv.KVFX_ENOSPACE
+    assert call(ctypes.byref(fast), 16, 16, 16, 16, groups, 2, 64, 32, 1024, 264, need, None) == kv.KVFX_EINVAL
+    # row-by-row shapes need none; refused arguments size none
+    assert kv.lib.kvfx_decode_shared_workspace_bytes(c, groups, 2, 4, 1024) == 0
+    assert kv.lib.kvfx_decode_shared_workspace_bytes(ctypes.byref(fast), groups, 2, 30, 1024) == 0
