@@ -209,6 +209,32 @@ __device__ __forceinline__ void tma_load_4d(void* smem_dst, const CUtensorMap* m
         : "memory");
 }
 
+// The same under an L2 cache policy (see l2_evict_first).
+__device__ __forceinline__ void tma_load_4d_hint(void* smem_dst, const CUtensorMap* map, int c0, int c1, int c2,
+                                                 int c3, uint64_t* bar, uint64_t policy) {
+    asm volatile(
+        "cp.async.bulk.tensor.4d.shared::cluster.global.tile.mbarrier::complete_tx::bytes.L2::cache_hint"
+        " [%0], [%1, {%2, %3, %4, %5}], [%6], %7;"
+        ::"r"(smem_addr(smem_dst)), "l"(map), "r"(c0), "r"(c1), "r"(c2), "r"(c3),
+          "r"(smem_addr(bar)), "l"(policy)
+        : "memory");
+}
+
+// Policy for data that is streamed through: its lines leave the L2 first, so
+// that a stream longer than the L2 does not push out what the kernels around
+// it need (lengths, tables, partial results, their code).
+__device__ __forceinline__ uint64_t l2_evict_first() {
+    uint64_t policy;
+    asm volatile("createpolicy.fractional.L2::evict_first.b64 %0, 1.0;" : "=l"(policy));
+    return policy;
+}
+
+__device__ __forceinline__ uint64_t l2_evict_normal() {
+    uint64_t policy;
+    asm volatile("createpolicy.fractional.L2::evict_normal.b64 %0, 1.0;" : "=l"(policy));
+    return policy;
+}
+
 // Tiled 3-D tensor store from shared memory, tracked as a bulk-async group:
 // commit with bulk_commit(), then bulk_wait_read<N>() returns once all but
 // the N most recent groups have finished reading shared memory, and

@@ -142,14 +142,16 @@ decode_mma_kernel(const __grid_constant__ DecodeParams p, const __grid_constant_
     // scheduled as soon as every CTA of this one has started (so its CTAs
     // take the SMs this launch's last wave leaves), and this one reads
     // nothing before the kernel ahead of it has completed.
-    pdl_allow_next();
     if constexpr (kTail) {
         // The prefix kernel lets this one start once its own wait is over, so
         // everything before it is complete; it writes nothing that is read
         // here. Every exit below waits for it all the same, so that the end
         // of this launch means the end of that one.
+        // (And the merge kernel may read the lengths before its own wait.)
         if (tail.after_prefix == 0) pdl_wait();
+        pdl_allow_next();
     } else {
+        pdl_allow_next();
         pdl_wait();
     }
     const uint64_t len = p.lens != nullptr ? p.lens[r] : p.single_len;
@@ -235,6 +237,8 @@ decode_mma_kernel(const __grid_constant__ DecodeParams p, const __grid_constant_
         if (lane < n_my) id_lo = append ? __ldcg(row + j0) : __ldg(row + j0);
         if (lane + 32 < n_my) id_hi = append ? __ldcg(row + j1) : __ldg(row + j1);
     }
+    uint64_t policy = 0;
+    if constexpr (kTail) policy = l2_evict_first();
     auto issue = [&](uint32_t i) {  // whole warp; lane 0 issues the copies of page i of this warp
         if (i >= n_my) return;
         const uint64_t j = pbeg + warp + static_cast<uint64_t>(kWarps) * i;
@@ -257,10 +261,17 @@ decode_mma_kernel(const __grid_constant__ DecodeParams p, const __grid_constant_
         mbar_arrive_expect_tx(&bars[warp][st], S::kStage);
 #pragma unroll
         for (int b = 0; b < S::kBoxes; ++b) {
-            tma_load_4d(kt + b * 2048, &kmap, b * 64, 0, static_cast<int>(kh), static_cast<int>(blk),
-                        &bars[warp][st]);
-            tma_load_4d(kt + S::kTile + b * 2048, &vmap, b * 64, 0, static_cast<int>(kh),
-                        static_cast<int>(blk), &bars[warp][st]);
+            if constexpr (kTail) {  // read once: keep it from pushing the pieces out of the L2
+                tma_load_4d_hint(kt + b * 2048, &kmap, b * 64, 0, static_cast<int>(kh), static_cast<int>(blk),
+                                 &bars[warp][st], policy);
+                tma_load_4d_hint(kt + S::kTile + b * 2048, &vmap, b * 64, 0, static_cast<int>(kh),
+                                 static_cast<int>(blk), &bars[warp][st], policy);
+            } else {
+                tma_load_4d(kt + b * 2048, &kmap, b * 64, 0, static_cast<int>(kh), static_cast<int>(blk),
+                            &bars[warp][st]);
+                tma_load_4d(kt + S::kTile + b * 2048, &vmap, b * 64, 0, static_cast<int>(kh),
+                            static_cast<int>(blk), &bars[warp][st]);
+            }
         }
     };
 #pragma unroll

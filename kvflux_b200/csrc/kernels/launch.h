@@ -182,6 +182,7 @@ struct PrefixArgs {
     const uint64_t* table;
     uint64_t max_blocks;
     uint32_t q_heads, grid;
+    bool stream;  // no group has more than one tile of query rows
     const PrefixGroups* groups;
     float* part_o;
     float* part_ml;
@@ -252,6 +253,10 @@ const CacheMaps* cache_maps(const CacheView& c, cudaError_t* err);
 // Unswizzled maps over the K and V caches, one box = one (page, head) tile of
 // block_size rows (the TMA gather's loads; cached per cache).
 const CacheMaps* gather_maps(const CacheView& c, cudaError_t* err);
+// Maps over the K and V caches for the prefix kernel (16-bit caches, hd a
+// multiple of 64, bs a multiple of 8): the cache as 8-row groups, each of
+// hd / 64 blocks of 8 rows x 128 bytes, one box = 2 groups, 128-byte swizzle.
+const CacheMaps* prefix_maps(const CacheView& c, cudaError_t* err);
 // Encodes a tiled, unswizzled tensor map (dims and box innermost first,
 // strides in bytes for dims 1..rank-1).
 bool encode_tiled(CUtensorMap* map, CUtensorMapDataType type, uint32_t rank, void* base, const uint64_t* dims,

@@ -106,6 +106,20 @@ bool encode_tiled(CUtensorMap* map, CUtensorMapDataType type, uint32_t rank, voi
 
 namespace {
 
+std::mutex g_prefix_mu;
+std::vector<Entry> g_prefix_entries;
+
+bool encode_groups(EncodeTiled fn, CUtensorMap* map, void* base, const CacheView& c) {
+    const CUtensorMapDataType t =
+        c.dtype == KVFX_BF16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16;
+    const cuuint64_t dims[4] = {64, 8, c.hd / 64, c.num_blocks * c.heads * (c.bs / 8)};
+    const cuuint64_t strides[3] = {c.row_bytes, 128, 8 * c.row_bytes};
+    const cuuint32_t box[4] = {64, 8, c.hd / 64, 2};
+    const cuuint32_t estr[4] = {1, 1, 1, 1};
+    return fn(map, t, 4, base, dims, strides, box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B,
+              CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+}
+
 struct GatherEntry {
     const void* k;
     const void* v;
@@ -117,6 +131,28 @@ std::mutex g_gather_mu;
 std::vector<GatherEntry> g_gather_entries;
 
 }  // namespace
+
+const CacheMaps* prefix_maps(const CacheView& c, cudaError_t* err) {
+    *err = cudaSuccess;
+    std::lock_guard<std::mutex> lock(g_prefix_mu);
+    for (const Entry& e : g_prefix_entries) {
+        if (e.k == c.k && e.v == c.v && e.num_blocks == c.num_blocks && e.heads == c.heads && e.bs == c.bs &&
+            e.hd == c.hd && e.dtype == c.dtype) {
+            return e.maps;
+        }
+    }
+    EncodeTiled fn = encoder(err);
+    if (fn == nullptr) return nullptr;
+    CacheMaps* m = new CacheMaps();
+    m->valid = encode_groups(fn, &m->k, c.k, c) && encode_groups(fn, &m->v, c.v, c);
+    if (!m->valid) {
+        delete m;
+        *err = cudaErrorInvalidValue;
+        return nullptr;
+    }
+    g_prefix_entries.push_back({c.k, c.v, c.num_blocks, c.heads, c.bs, c.hd, c.dtype, m});
+    return m;
+}
 
 const CacheMaps* gather_maps(const CacheView& c, cudaError_t* err) {
     *err = cudaSuccess;

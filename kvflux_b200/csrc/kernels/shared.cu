@@ -19,7 +19,7 @@ namespace kvfx {
 namespace {
 
 constexpr int kMergeWarps = 4;
-constexpr int kAhead = 4;  // pieces loaded before the first is joined
+constexpr uint32_t kAhead = 8;  // pieces' O in flight
 
 struct MergeParams {
     PrefixGroups groups;
@@ -29,6 +29,7 @@ struct MergeParams {
     const float* part_ml;
     const float* tail;     // tail splits: [row][heads x chunks][split][8][hd + 2]
     uint64_t max_len, max_blocks;
+    uint64_t tiles_inv;    // floor(2^64 / tiles)
     uint32_t grid;         // CTAs of the prefix launch
     uint32_t q_heads, kv_heads, q_group, chunks;
     uint32_t pages_per_split, max_splits;
@@ -40,87 +41,129 @@ template <int HD>
 __global__ void __launch_bounds__(kMergeWarps * 32) merge_kernel(const __grid_constant__ MergeParams p) {
     constexpr int kV = HD / 64;  // float2 per lane
     pdl_allow_next();
-    pdl_wait();
     const int lane = threadIdx.x & 31;
     const uint32_t id = blockIdx.x * kMergeWarps + (threadIdx.x >> 5);
     const uint32_t row = id / p.q_heads, j = id - row * p.q_heads;
-    if (row >= p.groups.rows()) return;
-    const uint64_t len = __ldg(p.lens + row);
-    if (len == 0) return;  // padding
+    // Nothing before the wait below reads what the launches ahead write (the
+    // lengths are older than both: see prefix.cu and the tail's order).
+    const bool inside = row < p.groups.rows();
+    const uint64_t len = inside ? __ldg(p.lens + row) : 0;
+    if (len == 0) {  // padding
+        pdl_wait();
+        return;
+    }
     const uint32_t g = p.groups.of_row(row);
     const uint32_t first = p.groups.pages[g];
     const uint64_t npages = ceil_div(len, 16);
     if (len > p.max_len || npages > p.max_blocks || len < static_cast<uint64_t>(first) * 16) {
         if (lane == 0) raise_flag(p.status, KVFX_FLAG_BAD_INDEX);
+        pdl_wait();
         return;
     }
+    // The row's pieces in order: its prefix segments, then its own splits.
+    const uint32_t kh = j / p.q_group, gq = j - kh * p.q_group;
+    uint32_t n_seg = 0;
+    uint64_t seg_row = 0;  // first segment's row of part_o
+    if (first != 0) {
+        const uint32_t row0 = g == 0 ? 0 : p.groups.row_end[g - 1];
+        const uint32_t tile0 = g == 0 ? 0 : p.groups.tile_end[g - 1], pair0 = g == 0 ? 0 : p.groups.pair_end[g - 1];
+        const uint32_t rows = (p.groups.row_end[g] - row0) * p.q_group;
+        const uint32_t m = (row - row0) * p.q_group + gq;  // query row in the group's matrix
+        const uint32_t pair = kh * ((rows + 127) / 128) + m / 128;
+        const uint32_t ntiles = (first + 7) / 8;
+        // The CTAs whose runs [tiles c / grid, tiles (c + 1) / grid) meet the pair's tiles.
+        const uint32_t tiles = p.groups.tiles(), t0 = tile0 + pair * ntiles;
+        auto owner = [&](uint32_t t) {
+            const uint64_t x = (static_cast<uint64_t>(t) + 1) * p.grid - 1;
+            uint64_t c = __umul64hi(x, p.tiles_inv);  // x / tiles, or one less
+            if (x - c * tiles >= tiles) ++c;
+            return static_cast<uint32_t>(c);
+        };
+        const uint32_t c0 = owner(t0);
+        n_seg = owner(t0 + ntiles - 1) - c0 + 1;
+        seg_row = static_cast<uint64_t>(c0 + pair0 + pair) * 128 + m % 128;
+    }
+    const uint32_t own_pages = static_cast<uint32_t>(npages) - first;
+    const uint32_t n = n_seg + (own_pages + p.pages_per_split - 1) / p.pages_per_split;
+    const uint64_t unit = static_cast<uint64_t>(row) * (p.kv_heads * p.chunks) + kh * p.chunks + gq / 8;
+    const float* tail = p.tail + (unit * p.max_splits * 8 + gq % 8) * (HD + 2);
+
     float M = -INFINITY, L = 0.f;
     float2 acc[kV];
 #pragma unroll
     for (int v = 0; v < kV; ++v) acc[v] = make_float2(0.f, 0.f);
-    // Joins up to kAhead pieces; piece i's (m, l) at ml(i) and O at o(i).
-    auto join = [&](uint32_t n, auto&& ml, auto&& o) {
-        float2 s[kAhead], x[kAhead][kV];
+    float2* out = reinterpret_cast<float2*>(p.o + (static_cast<uint64_t>(row) * p.q_heads + j) * HD);
+    // 32 pieces a pass, one a lane for (m, l) and the weights. A pass before
+    // the wait reads this row's own output in place of a piece and forgets it:
+    // it brings the loop's code and the kernel's parameters into the caches
+    // while the launches ahead run (they stream more K and V than the L2
+    // holds, so what is missing here would come from HBM, line after line).
+    uint32_t warm, base = 0;
+    asm volatile("mov.u32 %0, 0;" : "=r"(warm) : "r"(n));  // unknown to the compiler: one copy of the loop; n is there
+#pragma unroll 1
+    do {
+        const uint32_t here = warm != 0 ? min(32u, n - base) : 1u;
+        const uint32_t i = base + lane;
+        const uint64_t r = seg_row + static_cast<uint64_t>(i) * 128;
+        const float* split = tail + static_cast<int64_t>(static_cast<int32_t>(i - n_seg)) * 8 * (HD + 2);
+        const float* o = i < n_seg ? p.part_o + r * HD : split;
+        const float* at = i < n_seg ? p.part_ml + r * 2 : split + HD;
+        if (warm == 0) o = at = reinterpret_cast<const float*>(out);
+        float2 ml = make_float2(-INFINITY, 0.f);
+        if (lane < here) ml = __ldcg(reinterpret_cast<const float2*>(at));
+        float m_new = ml.x;
 #pragma unroll
-        for (uint32_t i = 0; i < kAhead; ++i) {
-            s[i] = make_float2(-INFINITY, 0.f);
-            if (i < n) {
-                s[i] = __ldcg(reinterpret_cast<const float2*>(ml(i)));
-#pragma unroll
-                for (int v = 0; v < kV; ++v) x[i][v] = __ldcg(reinterpret_cast<const float2*>(o(i)) + lane + 32 * v);
-            }
-        }
-        float m_new = M;
-#pragma unroll
-        for (uint32_t i = 0; i < kAhead; ++i) m_new = fmaxf(m_new, s[i].x);
-        // A piece without any visible score (m = -inf) weighs nothing.
+        for (int s = 16; s > 0; s >>= 1) m_new = fmaxf(m_new, __shfl_xor_sync(0xffffffffu, m_new, s));
+        m_new = fmaxf(m_new, M);
         const float keep = M == -INFINITY ? 0.f : exp2f(M - m_new);
         M = m_new;
-        L *= keep;
+        // A piece without any visible score (m = -inf) weighs nothing,
+        // whatever its O holds.
+        const float w = ml.x == -INFINITY ? 0.f : exp2f(ml.x - M);
+        float sum = w != 0.f ? ml.y * w : 0.f;
+#pragma unroll
+        for (int s = 16; s > 0; s >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, s);
+        L = fmaf(L, keep, sum);
 #pragma unroll
         for (int v = 0; v < kV; ++v) acc[v] = make_float2(acc[v].x * keep, acc[v].y * keep);
+        uint32_t k = 0;
+#pragma unroll 1
+        do {
+            float2 x[kAhead][kV];
+            float wa[kAhead];
 #pragma unroll
-        for (uint32_t i = 0; i < kAhead; ++i) {
-            if (i >= n || s[i].x == -INFINITY) continue;
-            const float w = exp2f(s[i].x - M);
-            L = fmaf(s[i].y, w, L);
+            for (uint32_t a = 0; a < kAhead; ++a) {
+                const uint64_t at = __shfl_sync(0xffffffffu, reinterpret_cast<uint64_t>(o), (k + a) & 31u);
+                wa[a] = __shfl_sync(0xffffffffu, w, (k + a) & 31u);
 #pragma unroll
-            for (int v = 0; v < kV; ++v) {
-                acc[v].x = fmaf(x[i][v].x, w, acc[v].x);
-                acc[v].y = fmaf(x[i][v].y, w, acc[v].y);
+                for (int v = 0; v < kV; ++v) {
+                    x[a][v] = make_float2(0.f, 0.f);
+                    if (k + a < here) x[a][v] = __ldcg(reinterpret_cast<const float2*>(at) + lane + 32 * v);
+                }
             }
+#pragma unroll
+            for (uint32_t a = 0; a < kAhead; ++a) {
+                if (wa[a] == 0.f) continue;  // (NaN from a piece that weighs nothing stays out)
+#pragma unroll
+                for (int v = 0; v < kV; ++v) {
+                    acc[v].x = fmaf(x[a][v].x, wa[a], acc[v].x);
+                    acc[v].y = fmaf(x[a][v].y, wa[a], acc[v].y);
+                }
+            }
+            k += kAhead;
+        } while (k < here);
+        if (warm != 0) {
+            base += 32;
+        } else {
+            warm = 1;
+            pdl_wait();
+            M = -INFINITY;
+            L = 0.f;
+#pragma unroll
+            for (int v = 0; v < kV; ++v) acc[v] = make_float2(0.f, 0.f);
         }
-    };
-
-    const uint32_t kh = j / p.q_group, gq = j - kh * p.q_group;
-    if (first != 0) {
-        const uint32_t row0 = g == 0 ? 0 : p.groups.row_end[g - 1];
-        const uint32_t tile0 = g == 0 ? 0 : p.groups.tile_end[g - 1], pair0 = g == 0 ? 0 : p.groups.pair_end[g - 1];
-        const uint32_t m = (row - row0) * p.q_group + gq;  // query row in the group's matrix
-        const uint32_t m_tiles = ((p.groups.row_end[g] - row0) * p.q_group + 127) / 128;
-        const uint32_t pair = kh * m_tiles + m / 128;
-        const uint32_t ntiles = (first + 7) / 8;
-        // The CTAs whose runs [tiles c / grid, tiles (c + 1) / grid) meet the pair's tiles.
-        const uint64_t tiles = p.groups.tiles(), t0 = tile0 + static_cast<uint64_t>(pair) * ntiles;
-        auto owner = [&](uint64_t t) { return static_cast<uint32_t>(((t + 1) * p.grid - 1) / tiles); };
-        const uint32_t c0 = owner(t0), n = owner(t0 + ntiles - 1) - c0 + 1;
-        const uint64_t base = (static_cast<uint64_t>(c0 + pair0 + pair)) * 128 + m % 128;
-        for (uint32_t s = 0; s < n; s += kAhead) {
-            join(min(n - s, static_cast<uint32_t>(kAhead)),
-                 [&](uint32_t i) { return p.part_ml + (base + static_cast<uint64_t>(s + i) * 128) * 2; },
-                 [&](uint32_t i) { return p.part_o + (base + static_cast<uint64_t>(s + i) * 128) * HD; });
-        }
-    }
-    const uint32_t n = static_cast<uint32_t>(ceil_div(npages - first, p.pages_per_split));
-    const uint64_t unit = static_cast<uint64_t>(row) * (p.kv_heads * p.chunks) + kh * p.chunks + gq / 8;
-    const float* tail = p.tail + (unit * p.max_splits * 8 + gq % 8) * (HD + 2);
-    for (uint32_t s = 0; s < n; s += kAhead) {
-        join(min(n - s, static_cast<uint32_t>(kAhead)),
-             [&](uint32_t i) { return tail + static_cast<uint64_t>(s + i) * 8 * (HD + 2) + HD; },
-             [&](uint32_t i) { return tail + static_cast<uint64_t>(s + i) * 8 * (HD + 2); });
-    }
+    } while (base < n);
     const float inv = 1.f / L;
-    float2* out = reinterpret_cast<float2*>(p.o + (static_cast<uint64_t>(row) * p.q_heads + j) * HD);
 #pragma unroll
     for (int v = 0; v < kV; ++v) out[lane + 32 * v] = make_float2(acc[v].x * inv, acc[v].y * inv);
 }
@@ -130,6 +173,7 @@ __global__ void __launch_bounds__(kMergeWarps * 32) merge_kernel(const __grid_co
 struct Plan {
     PrefixGroups groups;
     uint32_t grid;             // prefix CTAs (0: nothing shared)
+    bool stream;               // no group has more than one tile of query rows
     uint32_t pages_per_split;  // tail splits
     uint32_t max_splits;       // 0: no row has pages of its own
     uint64_t off_ml, off_tail, bytes;
@@ -137,7 +181,7 @@ struct Plan {
 
 bool fast_shape(const CacheView& c, uint32_t q_heads) {
     return (c.dtype == KVFX_BF16 || c.dtype == KVFX_F16) && c.bs == 16 && (c.hd == 64 || c.hd == 128) &&
-           c.num_blocks < (1ull << 31) && q_heads <= 65535;
+           c.num_blocks * c.heads < (1ull << 30) && q_heads <= 65535;
 }
 
 bool make_plan(const CacheView& c, const kvfx_prefix_group* groups, uint32_t n, uint32_t q_heads, uint64_t max_len,
@@ -146,6 +190,7 @@ bool make_plan(const CacheView& c, const kvfx_prefix_group* groups, uint32_t n, 
     const uint64_t q_group = q_heads / c.heads, max_pages = ceil_div(max_len, 16);
     if (max_pages >= (1ull << 31)) return false;
     PrefixGroups& gs = plan->groups;
+    plan->stream = true;
     gs.n = n;
     uint64_t rows = 0, pairs = 0, tiles = 0, tail_pages = 0;
     for (uint32_t g = 0; g < n; ++g) {
@@ -153,15 +198,18 @@ bool make_plan(const CacheView& c, const kvfx_prefix_group* groups, uint32_t n, 
         const uint64_t group_pairs = pages != 0 ? c.heads * ceil_div(groups[g].rows * q_group, 128) : 0;
         rows += groups[g].rows;
         pairs += group_pairs;
+        if (group_pairs > c.heads) plan->stream = false;
         tiles += group_pairs * ceil_div(pages, 8);
-        if (pairs >= (1ull << 31) || tiles >= (1ull << 31)) return false;
+        if (tiles >= (1ull << 31)) return false;
         tail_pages = std::max(tail_pages, max_pages - pages);
         gs.row_end[g] = static_cast<uint32_t>(rows);
         gs.pages[g] = static_cast<uint32_t>(pages);
         gs.pair_end[g] = static_cast<uint32_t>(pairs);
         gs.tile_end[g] = static_cast<uint32_t>(tiles);
     }
-    plan->grid = static_cast<uint32_t>(umin64(tiles, device_sm_count(c.device)));
+    // One CTA per SM; more where a run would pass the 256 tiles one CTA lists.
+    plan->grid = static_cast<uint32_t>(
+        umin64(tiles, std::max<uint64_t>(device_sm_count(c.device), ceil_div(tiles, 256))));
     plan->pages_per_split = 1;
     plan->max_splits = 0;
     if (tail_pages != 0) {
@@ -212,8 +260,10 @@ cudaError_t launch_decode_shared(const CacheView& c, const SharedArgs& a, unsign
     float* part_ml = reinterpret_cast<float*>(ws + plan.off_ml);
     float* tail = reinterpret_cast<float*>(ws + plan.off_tail);
     if (plan.grid != 0) {
-        const PrefixArgs pa{a.q, a.table, a.max_blocks, a.q_heads, plan.grid, &plan.groups, part_o, part_ml};
-        err = launch_prefix_tc(c, pa, *maps, status, s);
+        const PrefixArgs pa{a.q, a.table, a.max_blocks, a.q_heads, plan.grid, plan.stream, &plan.groups, part_o, part_ml};
+        const CacheMaps* groups = prefix_maps(c, &err);
+        if (groups == nullptr) return err != cudaSuccess ? err : cudaErrorInvalidValue;
+        err = launch_prefix_tc(c, pa, *groups, status, s);
         if (err != cudaSuccess) return err;
     }
     if (plan.max_splits != 0) {
@@ -232,6 +282,8 @@ cudaError_t launch_decode_shared(const CacheView& c, const SharedArgs& a, unsign
     m.max_len = a.max_len;
     m.max_blocks = a.max_blocks;
     m.grid = plan.grid;
+    const uint32_t tiles = plan.groups.tiles();
+    m.tiles_inv = tiles > 1 ? ~0ull / tiles + (~0ull % tiles == tiles - 1 ? 1 : 0) : ~0ull;
     m.q_heads = a.q_heads;
     m.kv_heads = c.heads;
     m.q_group = a.q_heads / c.heads;
