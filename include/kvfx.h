@@ -197,8 +197,8 @@ int kvfx_rotary_table(float* cos_sin, uint64_t max_positions, uint32_t rotary_di
  *   q_out     : device float[num_tokens][q_heads][head_size]
  * q_heads may be 0 (q and q_out are then not looked at). A token whose slot
  * or position is out of range is skipped and sets KVFX_FLAG_BAD_INDEX.
- * Rows of 32, 64, 128 or 256 elements with 16-byte aligned bases and strides,
- * and a rotary_dim that is a multiple of 16 (8 interleaved), take a kernel of
+ * Rows of 32, 64, 128 or 256 elements with 16-byte aligned bases and strides
+ * (q_out: 32-byte), and a rotary_dim that is a multiple of 16 (8 interleaved), take a kernel of
  * 16-byte vectors; other shapes an element-wise one.
  * No counterpart in the reference, whose write takes K and V as they are
  * (src/v2/paged_kv_write.cu:101-139).

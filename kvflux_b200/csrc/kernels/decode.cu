@@ -107,6 +107,7 @@ struct PrefixTail {
     uint32_t q_group;     // query heads per KV head
     uint32_t chunks;      // CTAs per KV head: ceil(q_group / 8)
     uint32_t after_prefix;  // launched as a dependent of the prefix kernel
+    uint32_t direct;        // no prefix kernel and one split a row: its pages from the first on, O written here
 };
 
 template <int HD, typename T, typename Tail>
@@ -156,13 +157,26 @@ decode_mma_kernel(const __grid_constant__ DecodeParams p, const __grid_constant_
     }
     const uint64_t len = p.lens != nullptr ? p.lens[r] : p.single_len;
     const uint64_t npages = ceil_div(len, 16);
-    uint64_t first = 0;  // the row's first page here
+    uint64_t first = 0;   // the row's first page here
+    uint64_t shared = 0;  // pages that the group's first row names
+    const uint64_t* row0 = nullptr;
     if constexpr (kTail) {
-        first = tail.groups.pages[tail.groups.of_row(static_cast<uint32_t>(r))];
-        // Rows outside the bounds are refused (and flagged) by the merge kernel.
-        if (len > tail.max_len || npages <= first) {
-            pdl_wait();
-            return;
+        const uint32_t g = tail.groups.of_row(static_cast<uint32_t>(r));
+        const uint64_t pages = tail.groups.pages[g];
+        if (tail.direct != 0) {
+            if (len != 0 && (len > tail.max_len || npages > p.max_blocks || len < pages * 16)) {
+                if (tid == 0) raise_flag(p.status, KVFX_FLAG_BAD_INDEX);
+                return;
+            }
+            shared = pages;
+            row0 = p.table + static_cast<uint64_t>(g == 0 ? 0 : tail.groups.row_end[g - 1]) * p.max_blocks;
+        } else {
+            first = pages;
+            // Rows outside the bounds are refused (and flagged) by the merge kernel.
+            if (len > tail.max_len || npages <= first) {
+                pdl_wait();
+                return;
+            }
         }
     }
     const uint32_t nsplits = static_cast<uint32_t>(ceil_div(npages - first, p.pages_per_split));
@@ -234,8 +248,8 @@ decode_mma_kernel(const __grid_constant__ DecodeParams p, const __grid_constant_
     if (ids_cached) {
         const uint64_t j0 = pbeg + warp + static_cast<uint64_t>(kWarps) * lane;
         const uint64_t j1 = j0 + static_cast<uint64_t>(kWarps) * 32;
-        if (lane < n_my) id_lo = append ? __ldcg(row + j0) : __ldg(row + j0);
-        if (lane + 32 < n_my) id_hi = append ? __ldcg(row + j1) : __ldg(row + j1);
+        if (lane < n_my) id_lo = append ? __ldcg(row + j0) : __ldg((kTail && j0 < shared ? row0 : row) + j0);
+        if (lane + 32 < n_my) id_hi = append ? __ldcg(row + j1) : __ldg((kTail && j1 < shared ? row0 : row) + j1);
     }
     uint64_t policy = 0;
     if constexpr (kTail) policy = l2_evict_first();
@@ -246,7 +260,7 @@ decode_mma_kernel(const __grid_constant__ DecodeParams p, const __grid_constant_
         if (ids_cached) {
             blk = __shfl_sync(0xffffffffu, i < 32 ? id_lo : id_hi, i & 31);
         } else if (lane == 0) {
-            blk = append ? __ldcg(row + j) : __ldg(row + j);
+            blk = append ? __ldcg(row + j) : __ldg((kTail && j < shared ? row0 : row) + j);
         } else {
             blk = 0;
         }
@@ -414,7 +428,9 @@ decode_mma_kernel(const __grid_constant__ DecodeParams p, const __grid_constant_
     // A load never arrived (status already flagged): no O from this CTA; a
     // split still counts itself with an empty partial (below).
     const bool failed = s_flag != 0;
-    if (!kTail && failed && nsplits == 1) return;
+    bool alone = nsplits == 1;  // this CTA writes O
+    if constexpr (kTail) alone = tail.direct != 0;
+    if (failed && alone) return;
 
     float* mo = reinterpret_cast<float*>(smem);  // [kWarps][8][HD]
     if (!failed) {
@@ -451,13 +467,15 @@ decode_mma_kernel(const __grid_constant__ DecodeParams p, const __grid_constant_
     __syncthreads();
 
     const uint64_t pair = r * (kTail ? gridDim.y : p.kv_heads) + (kTail ? blockIdx.y : kh);
-    if (!kTail && nsplits == 1) {
+    if (alone) {
         for (uint32_t idx = tid; idx < G * HD; idx += kWarps * 32) {
             const uint32_t gg = idx / HD, d = idx - gg * HD;
             float acc = 0.f;
 #pragma unroll
             for (int w = 0; w < kWarps; ++w) acc += mo[(w * 8 + gg) * HD + d] * s_scale[w][gg];
-            p.o[(r * p.kv_heads * G + static_cast<uint64_t>(kh) * G + gg) * HD + d] = acc * s_inv[gg];
+            uint32_t q_heads = p.kv_heads * p.group;
+            if constexpr (kTail) q_heads = p.kv_heads * tail.q_group;
+            p.o[(r * q_heads + qh0 + gg) * HD + d] = acc * s_inv[gg];
         }
         return;
     }
@@ -619,6 +637,7 @@ cudaError_t launch_tail(const CacheView& c, const TailArgs& a, const CacheMaps* 
     }
     DecodeParams p{};
     p.q = a.q;
+    p.o = a.o;
     p.table = a.table;
     p.lens = a.lens;
     p.max_blocks = a.max_blocks;
@@ -630,7 +649,7 @@ cudaError_t launch_tail(const CacheView& c, const TailArgs& a, const CacheMaps* 
     p.partial = a.partial;
     p.status = status;
     const uint32_t q_group = a.q_heads / c.heads, chunks = (q_group + 7) / 8;
-    const PrefixTail tail{*a.groups, a.max_len, q_group, chunks, a.after_prefix ? 1u : 0u};
+    const PrefixTail tail{*a.groups, a.max_len, q_group, chunks, a.after_prefix ? 1u : 0u, a.direct ? 1u : 0u};
     cudaLaunchConfig_t cfg{};
     cfg.gridDim = dim3(a.max_splits, c.heads * chunks, a.groups->rows());
     cfg.blockDim = dim3(kWarps * 32);

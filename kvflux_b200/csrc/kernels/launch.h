@@ -156,16 +156,18 @@ struct PrefixGroups {
 
 // The rows' own pages behind their groups' prefixes (decode.cu, tail mode):
 // split s of (row, KV head and chunk y) leaves its partial, 8 (hd + 2)
-// floats, at partial[((row * gridDim.y + y) * max_splits + s)].
+// floats, at partial[((row * gridDim.y + y) * max_splits + s)]. `direct`: all
+// of a row's pages instead, in one split whose O goes to o.
 struct TailArgs {
     const float* q;
+    float* o;
     const uint64_t* table;
     const uint64_t* lens;
     uint64_t max_blocks, max_len;
     uint32_t q_heads, pages_per_split, max_splits;
     const PrefixGroups* groups;
     float* partial;
-    bool after_prefix;
+    bool after_prefix, direct;
 };
 // A split size the kernel takes, near `pps`, for rows of at most max_pages.
 uint32_t decode_tail_split(const CacheView& c, uint64_t max_pages, uint32_t pps);

@@ -13,9 +13,11 @@
 // Bounded by HBM for a prefill chunk (each input read once, each output
 // written once) and by memory latency for a decode step. A group of lanes
 // holds one head's row, eight elements a lane, and walks the token's heads
-// with the token's cosines and sines in registers; all of a pass's rows are
-// loaded before the first is used. The norm's sum and the rotation's partner
-// dims move by shuffles inside the group.
+// with the token's factors in registers; a pass's rows are loaded while the
+// pass before is computed. The norm's sum and the rotation's partner dims
+// move by shuffles inside the group. B200, 8192 tokens of 32 + 8 + 8 heads of
+// 128 bf16: 49 us, 5.6 TB/s (57 us with 64 threads a CTA, 71 us with 128, 60 us
+// without the pass ahead); a decode step's 64 tokens: 3.6 us.
 #include <algorithm>
 #include <cmath>
 
@@ -25,9 +27,11 @@
 namespace kvfx {
 namespace {
 
-constexpr int kThreads = 128;
-constexpr int kEl = 8;    // elements per lane
-constexpr int kRows = 4;  // rows in flight per lane group
+constexpr int kThreads = 32;      // one warp a CTA: many small ones hide the chain of loads a token has
+constexpr int kMinCtas = 18;      // per SM (112 registers)
+constexpr int kAnyThreads = 128;  // of the element-wise kernel
+constexpr int kEl = 8;            // elements per lane
+constexpr int kRows = 4;          // rows in flight per lane group, and as many behind them
 
 struct RotatedParams {
     const char* q;
@@ -48,49 +52,74 @@ struct RotatedParams {
     unsigned* status;
 };
 
+// A lane's eight elements as they are stored.
 template <typename T>
-__device__ __forceinline__ void load8(const T* p, uint4 (&raw)[sizeof(T) / 2]) {
+struct Raw {
+    uint4 w[sizeof(T) / 2];
+};
+
+template <typename T>
+__device__ __forceinline__ Raw<T> load8(const T* p) {
+    Raw<T> r;
 #pragma unroll
-    for (int i = 0; i < static_cast<int>(sizeof(T) / 2); ++i) raw[i] = __ldg(reinterpret_cast<const uint4*>(p) + i);
+    for (int i = 0; i < static_cast<int>(sizeof(T) / 2); ++i) r.w[i] = __ldg(reinterpret_cast<const uint4*>(p) + i);
+    return r;
 }
 
 template <typename T>
-__device__ __forceinline__ void widen8(const uint4 (&raw)[sizeof(T) / 2], float (&x)[kEl]) {
-    const T* e = reinterpret_cast<const T*>(raw);
+__device__ __forceinline__ void store8(T* p, const Raw<T>& r) {
 #pragma unroll
-    for (int i = 0; i < kEl; ++i) x[i] = Elem<T>::to_f32(e[i]);
+    for (int i = 0; i < static_cast<int>(sizeof(T) / 2); ++i) reinterpret_cast<uint4*>(p)[i] = r.w[i];
 }
 
+// Pairs (2i, 2i + 1) of the elements as packed floats.
 template <typename T>
-__device__ __forceinline__ void narrow8(const float (&x)[kEl], uint4 (&raw)[sizeof(T) / 2]) {
-    if constexpr (sizeof(T) == 2) {
-        uint32_t w[4];
+__device__ __forceinline__ void widen8(const Raw<T>& r, uint64_t (&x)[kEl / 2]) {
+    const uint32_t* u = reinterpret_cast<const uint32_t*>(r.w);
 #pragma unroll
-        for (int i = 0; i < 4; ++i) w[i] = Elem<T>::pack(x[2 * i], x[2 * i + 1]);
-        raw[0] = make_uint4(w[0], w[1], w[2], w[3]);
-    } else {
-#pragma unroll
-        for (int i = 0; i < 2; ++i)
-            raw[i] = make_uint4(__float_as_uint(x[4 * i]), __float_as_uint(x[4 * i + 1]),
-                                __float_as_uint(x[4 * i + 2]), __float_as_uint(x[4 * i + 3]));
+    for (int i = 0; i < kEl / 2; ++i) {
+        if constexpr (sizeof(T) == 2) x[i] = widen2<T>(u[i]);
+        else x[i] = f2_pack(__uint_as_float(u[2 * i]), __uint_as_float(u[2 * i + 1]));
     }
 }
 
 template <typename T>
-__device__ __forceinline__ void store8(T* p, const uint4 (&raw)[sizeof(T) / 2]) {
+__device__ __forceinline__ Raw<T> narrow8(const uint64_t (&x)[kEl / 2]) {
+    Raw<T> r;
+    uint32_t* u = reinterpret_cast<uint32_t*>(r.w);
 #pragma unroll
-    for (int i = 0; i < static_cast<int>(sizeof(T) / 2); ++i) reinterpret_cast<uint4*>(p)[i] = raw[i];
+    for (int i = 0; i < kEl / 2; ++i) {
+        float a, b;
+        f2_unpack(x[i], a, b);
+        if constexpr (sizeof(T) == 2) {
+            u[i] = Elem<T>::pack(a, b);
+        } else {
+            u[2 * i] = __float_as_uint(a);
+            u[2 * i + 1] = __float_as_uint(b);
+        }
+    }
+    return r;
 }
 
-__device__ __forceinline__ void load_f8(const float* p, float (&x)[kEl]) {
+__device__ __forceinline__ uint64_t f2_swap(uint64_t x) {
+    float a, b;
+    f2_unpack(x, a, b);
+    return f2_pack(b, a);
+}
+
+__device__ __forceinline__ void load_f8(const float* p, uint64_t (&x)[kEl / 2]) {
 #pragma unroll
     for (int i = 0; i < kEl / 4; ++i) {
         const float4 a = __ldg(reinterpret_cast<const float4*>(p) + i);
-        x[4 * i] = a.x;
-        x[4 * i + 1] = a.y;
-        x[4 * i + 2] = a.z;
-        x[4 * i + 3] = a.w;
+        x[2 * i] = f2_pack(a.x, a.y);
+        x[2 * i + 1] = f2_pack(a.z, a.w);
     }
+}
+
+// 32 contiguous bytes in one store.
+__device__ __forceinline__ void store_f8(float* p, const uint64_t (&x)[kEl / 2]) {
+    asm volatile("st.global.v4.b64 [%0], {%1, %2, %3, %4};" ::"l"(p), "l"(x[0]), "l"(x[1]), "l"(x[2]), "l"(x[3])
+                 : "memory");
 }
 
 // Where token t goes: false for a padding token (KVFX_NO_SLOT) and, with the
@@ -106,144 +135,173 @@ __device__ __forceinline__ bool token_place(const RotatedParams& p, uint64_t t, 
     return true;
 }
 
+// Element offset of head 0's row of a slot in a cache (head h: + h * bs * hd).
+__device__ __forceinline__ uint64_t slot_row(const RotatedParams& p, uint64_t slot) {
+    const uint64_t page = (p.bs & (p.bs - 1)) == 0 ? slot >> (31 - __clz(static_cast<int>(p.bs))) : slot / p.bs;
+    return (page * p.kv_heads * p.bs + (slot - page * p.bs)) * p.hd;
+}
+
 // LPR lanes per row (head_size = 8 LPR). One CTA per token and slice of its
 // rows (blockIdx.y of gridDim.y); rows are Q heads, K heads, V heads in turn.
+// With weight and rotation folded into two factors per dimension, a row is
+//     y_d = (x_d a_d + x_partner(d) b_d) / sqrt(mean(x^2) + eps),
+// a = w c and b = +- w_partner s, and the partner's x comes as stored (16-bit
+// rows: four shuffles a row, and half the instructions of norming first).
 template <typename T, int LPR>
-__global__ void __launch_bounds__(kThreads) write_rotated_kernel(const __grid_constant__ RotatedParams p) {
+__global__ void __launch_bounds__(kThreads, kMinCtas) write_rotated_kernel(const __grid_constant__ RotatedParams p) {
     constexpr int kGroups = kThreads / LPR;
     constexpr int kHd = LPR * kEl;
     pdl_allow_next();
     pdl_wait();  // launched as a dependent: the previous kernel's writes first
     const uint64_t t = blockIdx.x;
     const int l = threadIdx.x % LPR, g = threadIdx.x / LPR;
-    const uint32_t rows = p.q_heads + 2 * p.kv_heads;
+    const uint32_t rows = p.q_heads + 2 * p.kv_heads, first_v = p.q_heads + p.kv_heads;
     const uint32_t first = blockIdx.y * kGroups + g, step = gridDim.y * kGroups;
     const int d0 = l * kEl;
+    // Shuffles stay inside a row's lanes: the rows of a warp may differ.
+    const uint32_t lanes = LPR == 32 ? 0xffffffffu : ((1u << LPR) - 1) << (threadIdx.x & 31 & ~(LPR - 1));
 
     auto row_ptr = [&](uint32_t r) {
         const T* base = reinterpret_cast<const T*>(p.q) + t * p.q_stride;
         uint32_t h = r;
-        if (r >= p.q_heads + p.kv_heads) {
+        if (r >= first_v) {
             base = reinterpret_cast<const T*>(p.v) + t * p.v_stride;
-            h = r - p.q_heads - p.kv_heads;
+            h = r - first_v;
         } else if (r >= p.q_heads) {
             base = reinterpret_cast<const T*>(p.k) + t * p.k_stride;
             h = r - p.q_heads;
         }
         return base + static_cast<uint64_t>(h) * kHd + d0;
     };
-    uint4 raw[kRows][sizeof(T) / 2];
-    auto load_rows = [&](uint32_t r0) {
+    Raw<T> raw[kRows], next[kRows];
+    auto load_rows = [&](uint32_t r0, Raw<T>(&to)[kRows]) {
 #pragma unroll
         for (int i = 0; i < kRows; ++i) {
-            const uint32_t r = r0 + i * step;
-            if (r < rows) load8(row_ptr(r), raw[i]);
+            if (r0 + i * step < rows) to[i] = load8(row_ptr(r0 + i * step));
         }
     };
-    load_rows(first);  // independent of the token's place: both latencies overlap
+    load_rows(first, raw);  // independent of the token's place: both latencies overlap
     uint64_t pos, slot;
     if (!token_place(p, t, pos, slot)) return;
 
-    // This lane's rotation: y = x * c + partner * s.
+    // This lane's factors for Q and for K rows, and where its partner dims are.
     const int rot = static_cast<int>(p.rotary_dim), half = rot / 2;
-    float c[kEl], s[kEl];
+    uint64_t qa[kEl / 2], qb[kEl / 2], ka[kEl / 2], kb[kEl / 2];
     int partner = l;
-    const float* tab = p.cos_sin + pos * p.rotary_dim;
+    {
+        const float* tab = p.cos_sin + pos * p.rotary_dim;
+        uint64_t c[kEl / 2], s[kEl / 2];
 #pragma unroll
-    for (int i = 0; i < kEl; ++i) {
-        c[i] = 1.f;
-        s[i] = 0.f;
-    }
-    if (p.interleaved) {  // pairs (2i, 2i + 1): four angles, partner in the same lane
-        if (d0 < rot) {
+        for (int i = 0; i < kEl / 2; ++i) {
+            c[i] = f2_pack(1.f, 1.f);
+            s[i] = 0;
+        }
+        if (d0 < rot && p.interleaved) {  // pairs (2i, 2i + 1): four angles, partner in the same lane
             const float4 cc = __ldg(reinterpret_cast<const float4*>(tab + d0 / 2));
             const float4 ss = __ldg(reinterpret_cast<const float4*>(tab + half + d0 / 2));
-            c[0] = c[1] = cc.x, c[2] = c[3] = cc.y, c[4] = c[5] = cc.z, c[6] = c[7] = cc.w;
-            s[0] = -ss.x, s[1] = ss.x, s[2] = -ss.y, s[3] = ss.y;
-            s[4] = -ss.z, s[5] = ss.z, s[6] = -ss.w, s[7] = ss.w;
-        }
-    } else if (d0 < rot) {  // pairs (i, i + rot / 2): the partner lane holds the other half
-        const bool low = d0 < half;
-        partner = low ? l + half / kEl : l - half / kEl;
-        const int a0 = low ? d0 : d0 - half;
-        load_f8(tab + a0, c);
-        load_f8(tab + half + a0, s);
-        if (low) {
+            c[0] = f2_pack(cc.x, cc.x), c[1] = f2_pack(cc.y, cc.y);
+            c[2] = f2_pack(cc.z, cc.z), c[3] = f2_pack(cc.w, cc.w);
+            s[0] = f2_pack(-ss.x, ss.x), s[1] = f2_pack(-ss.y, ss.y);
+            s[2] = f2_pack(-ss.z, ss.z), s[3] = f2_pack(-ss.w, ss.w);
+        } else if (d0 < rot) {  // pairs (i, i + rot / 2): the partner lane holds the other half
+            const bool low = d0 < half;
+            partner = low ? l + half / kEl : l - half / kEl;
+            const int a0 = low ? d0 : d0 - half;
+            load_f8(tab + a0, c);
+            load_f8(tab + half + a0, s);
+            const uint64_t sign = low ? f2_pack(-1.f, -1.f) : f2_pack(1.f, 1.f);
 #pragma unroll
-            for (int i = 0; i < kEl; ++i) s[i] = -s[i];
+            for (int i = 0; i < kEl / 2; ++i) s[i] = f2_mul(s[i], sign);
         }
+        auto fold = [&](const float* weight, uint64_t (&a)[kEl / 2], uint64_t (&b)[kEl / 2]) {
+#pragma unroll
+            for (int i = 0; i < kEl / 2; ++i) {
+                a[i] = c[i];
+                b[i] = s[i];
+            }
+            if (weight == nullptr) return;
+            uint64_t w[kEl / 2], wp[kEl / 2];
+            load_f8(weight + d0, w);
+            load_f8(weight + partner * kEl, wp);
+#pragma unroll
+            for (int i = 0; i < kEl / 2; ++i) {
+                a[i] = f2_mul(a[i], w[i]);
+                b[i] = f2_mul(b[i], p.interleaved ? f2_swap(wp[i]) : wp[i]);
+            }
+        };
+        fold(p.q_weight, qa, qb);
+        fold(p.k_weight, ka, kb);
     }
-    float wq[kEl], wk[kEl];
-    if (p.q_weight != nullptr) load_f8(p.q_weight + d0, wq);
-    if (p.k_weight != nullptr) load_f8(p.k_weight + d0, wk);
+    const uint64_t dst0 = slot_row(p, slot) + d0, head_step = static_cast<uint64_t>(p.bs) * kHd;
 
-    const uint64_t page = slot / p.bs, off = slot - page * p.bs;
-    // Rows in passes of kRows per group; every lane takes the same number of
-    // passes (shuffles below), rows past the end are not stored.
-    for (uint32_t r0 = first; r0 - g < rows; r0 += kRows * step) {
-        if (r0 != first) load_rows(r0);
+#pragma unroll 1
+    for (uint32_t r0 = first; r0 < rows; r0 += kRows * step) {
+        load_rows(r0 + kRows * step, next);  // in flight while this pass is computed
 #pragma unroll
         for (int i = 0; i < kRows; ++i) {
             const uint32_t r = r0 + i * step;
-            const bool is_v = r >= p.q_heads + p.kv_heads, is_k = !is_v && r >= p.q_heads;
-            if (r - g >= rows) break;  // past the end for every lane of the CTA
-            float x[kEl], y[kEl];
+            if (r >= rows) break;
+            if (r >= first_v) {
+                store8(reinterpret_cast<T*>(p.v_cache) + dst0 + (r - first_v) * head_step, raw[i]);
+                continue;
+            }
+            const bool is_k = r >= p.q_heads;
+            uint64_t x[kEl / 2], y[kEl / 2];
             widen8<T>(raw[i], x);
-            const float* weight = is_k ? p.k_weight : p.q_weight;
-            float sum = 0.f;
+            float scale = 1.f;
+            if ((is_k ? p.k_weight : p.q_weight) != nullptr) {
+                uint64_t sum2 = f2_mul(x[0], x[0]);
 #pragma unroll
-            for (int e = 0; e < kEl; ++e) sum = fmaf(x[e], x[e], sum);
+                for (int e = 1; e < kEl / 2; ++e) sum2 = f2_fma(x[e], x[e], sum2);
+                float sum, other;
+                f2_unpack(sum2, sum, other);
+                sum += other;
 #pragma unroll
-            for (int m = LPR / 2; m > 0; m >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, m);
-            if (weight != nullptr) {
-                const float scale = rsqrtf(fmaf(sum, p.inv_hd, p.eps));
-#pragma unroll
-                for (int e = 0; e < kEl; ++e) x[e] = x[e] * scale * (is_k ? wk[e] : wq[e]);
+                for (int m = LPR / 2; m > 0; m >>= 1) sum += __shfl_xor_sync(lanes, sum, m);
+                scale = rsqrtf(fmaf(sum, p.inv_hd, p.eps));
             }
             if (p.interleaved) {
 #pragma unroll
-                for (int e = 0; e < kEl; ++e) y[e] = fmaf(x[e], c[e], x[e ^ 1] * s[e]);
+                for (int e = 0; e < kEl / 2; ++e) y[e] = f2_swap(x[e]);
             } else {
+                Raw<T> other;
+                uint32_t* to = reinterpret_cast<uint32_t*>(other.w);
+                const uint32_t* from = reinterpret_cast<const uint32_t*>(raw[i].w);
 #pragma unroll
-                for (int e = 0; e < kEl; ++e) {
-                    const float other = __shfl_sync(0xffffffffu, x[e], partner, LPR);
-                    y[e] = fmaf(x[e], c[e], other * s[e]);
-                }
+                for (int e = 0; e < static_cast<int>(sizeof(Raw<T>) / 4); ++e) to[e] = __shfl_sync(lanes, from[e], partner, LPR);
+                widen8<T>(other, y);
             }
-            if (r >= rows) continue;
-            if (r < p.q_heads) {
-                float4* out = reinterpret_cast<float4*>(p.q_out + (t * p.q_heads + r) * kHd + d0);
-                out[0] = make_float4(y[0], y[1], y[2], y[3]);
-                out[1] = make_float4(y[4], y[5], y[6], y[7]);
-                continue;
+            const uint64_t scale2 = f2_pack(scale, scale);
+#pragma unroll
+            for (int e = 0; e < kEl / 2; ++e) {
+                const uint64_t b = f2_mul(y[e], is_k ? kb[e] : qb[e]);
+                y[e] = f2_mul(f2_fma(x[e], is_k ? ka[e] : qa[e], b), scale2);
             }
-            const uint32_t h = r - p.q_heads - (is_v ? p.kv_heads : 0);
-            const uint64_t dst = ((page * p.kv_heads + h) * p.bs + off) * kHd + d0;
-            if (is_v) {
-                store8(reinterpret_cast<T*>(p.v_cache) + dst, raw[i]);
+            if (is_k) {
+                store8(reinterpret_cast<T*>(p.k_cache) + dst0 + (r - p.q_heads) * head_step, narrow8<T>(y));
             } else {
-                uint4 k8[sizeof(T) / 2];
-                narrow8<T>(y, k8);
-                store8(reinterpret_cast<T*>(p.k_cache) + dst, k8);
+                store_f8(p.q_out + (t * p.q_heads + r) * kHd + d0, y);
             }
         }
+#pragma unroll
+        for (int i = 0; i < kRows; ++i) raw[i] = next[i];
     }
 }
 
 // Any head size, rotary_dim and alignment: one warp per row, element by
 // element; the partner element is read again (from L1).
 template <typename T>
-__global__ void __launch_bounds__(kThreads) write_rotated_any_kernel(const __grid_constant__ RotatedParams p) {
+__global__ void __launch_bounds__(kAnyThreads) write_rotated_any_kernel(const __grid_constant__ RotatedParams p) {
     pdl_allow_next();
     pdl_wait();
     const int lane = threadIdx.x & 31;
     const uint64_t t = blockIdx.x;
     uint64_t pos, slot;
     if (!token_place(p, t, pos, slot)) return;
-    const uint64_t page = slot / p.bs, off = slot - page * p.bs;
+    const uint64_t dst0 = slot_row(p, slot);
     const float* tab = p.cos_sin + pos * p.rotary_dim;
     const uint32_t rot = p.rotary_dim, half = rot / 2, rows = p.q_heads + 2 * p.kv_heads;
-    constexpr uint32_t kWarps = kThreads / 32;
+    constexpr uint32_t kWarps = kAnyThreads / 32;
     for (uint32_t r = blockIdx.y * kWarps + threadIdx.x / 32; r < rows; r += gridDim.y * kWarps) {
         const bool is_v = r >= p.q_heads + p.kv_heads, is_k = !is_v && r >= p.q_heads;
         const uint32_t h = is_v ? r - p.q_heads - p.kv_heads : is_k ? r - p.q_heads : r;
@@ -251,7 +309,7 @@ __global__ void __launch_bounds__(kThreads) write_rotated_any_kernel(const __gri
                      : is_k ? reinterpret_cast<const T*>(p.k) + t * p.k_stride
                             : reinterpret_cast<const T*>(p.q) + t * p.q_stride;
         x += static_cast<uint64_t>(h) * p.hd;
-        const uint64_t dst = ((page * p.kv_heads + h) * p.bs + off) * p.hd;
+        const uint64_t dst = dst0 + static_cast<uint64_t>(h) * p.bs * p.hd;
         if (is_v) {
             for (uint32_t d = lane; d < p.hd; d += 32) reinterpret_cast<T*>(p.v_cache)[dst + d] = x[d];
             continue;
@@ -337,11 +395,12 @@ cudaError_t launch_t(const RotatedParams& p, uint64_t n, bool vec, int sms, cuda
         }
     }
     const uint32_t rows = p.q_heads + 2 * p.kv_heads;
-    const dim3 grid(static_cast<uint32_t>(n), row_slices(n, rows, kThreads / 32, sms));
-    return launch_dependent(write_rotated_any_kernel<T>, grid, dim3(kThreads), s, p);
+    const dim3 grid(static_cast<uint32_t>(n), row_slices(n, rows, kAnyThreads / 32, sms));
+    return launch_dependent(write_rotated_any_kernel<T>, grid, dim3(kAnyThreads), s, p);
 }
 
 bool aligned16(const void* p) { return reinterpret_cast<uintptr_t>(p) % 16 == 0; }
+bool aligned32(const void* p) { return reinterpret_cast<uintptr_t>(p) % 32 == 0; }
 
 }  // namespace
 
@@ -373,7 +432,7 @@ cudaError_t launch_write_rotated(const CacheView& c, const kvfx_rotary& rotary, 
     const bool vec = (c.hd == 32 || c.hd == 64 || c.hd == 128 || c.hd == 256) &&
                      rotary.rotary_dim % (rotary.interleaved ? kEl : 2 * kEl) == 0 && a.q_stride % unit == 0 &&
                      a.k_stride % unit == 0 && a.v_stride % unit == 0 && aligned16(a.q) && aligned16(a.k) &&
-                     aligned16(a.v) && aligned16(a.q_out) && aligned16(c.k) && aligned16(c.v) &&
+                     aligned16(a.v) && aligned32(a.q_out) && aligned16(c.k) && aligned16(c.v) &&
                      aligned16(rotary.cos_sin) && aligned16(rotary.q_weight) && aligned16(rotary.k_weight);
     const int sms = device_sm_count(c.device);
     for (uint64_t i = 0; i < a.tokens; i += kMaxTokens) {

@@ -172,6 +172,7 @@ __global__ void __launch_bounds__(kMergeWarps * 32) merge_kernel(const __grid_co
 // size and the launches must agree on it).
 struct Plan {
     PrefixGroups groups;
+    bool direct;               // one launch, each row reading all of its pages
     uint32_t grid;             // prefix CTAs (0: nothing shared)
     bool stream;               // no group has more than one tile of query rows
     uint32_t pages_per_split;  // tail splits
@@ -206,6 +207,21 @@ bool make_plan(const CacheView& c, const kvfx_prefix_group* groups, uint32_t n, 
         gs.pages[g] = static_cast<uint32_t>(pages);
         gs.pair_end[g] = static_cast<uint32_t>(pairs);
         gs.tile_end[g] = static_cast<uint32_t>(tiles);
+    }
+    // Short rows: one launch, in which every row reads all of its pages (the
+    // shared ones from the L2), ends before three that share them. B200, us
+    // in a graph, 4 rows x 8 heads: 5.9 against 10.0 at 144 tokens, 7.5 / 10.0
+    // at 272, 10.5 / 10.2 at 528 (where the two launches saved on the host
+    // decide), 16.5 / 11.2 at 1040; as long as one wave of CTAs holds them
+    // (64 rows x 32 heads: 16.3 / 16.2 at 272, 23.4 / 17.5 at 528).
+    plan->direct = max_pages <= 40 && rows * c.heads * ceil_div(q_group, 8) <=
+                                          3 * static_cast<uint64_t>(device_sm_count(c.device));
+    if (plan->direct) {
+        plan->grid = 0;
+        plan->pages_per_split = decode_tail_split(c, max_pages, static_cast<uint32_t>(max_pages));
+        plan->max_splits = 1;
+        plan->off_ml = plan->off_tail = plan->bytes = 0;
+        return true;
     }
     // One CTA per SM; more where a run would pass the 256 tiles one CTA lists.
     plan->grid = static_cast<uint32_t>(
@@ -267,10 +283,10 @@ cudaError_t launch_decode_shared(const CacheView& c, const SharedArgs& a, unsign
         if (err != cudaSuccess) return err;
     }
     if (plan.max_splits != 0) {
-        const TailArgs ta{a.q, a.table, a.lens, a.max_blocks, a.max_len, a.q_heads, plan.pages_per_split,
-                          plan.max_splits, &plan.groups, tail, plan.grid != 0};
+        const TailArgs ta{a.q, a.o, a.table, a.lens, a.max_blocks, a.max_len, a.q_heads, plan.pages_per_split,
+                          plan.max_splits, &plan.groups, tail, plan.grid != 0, plan.direct};
         err = launch_decode_tail(c, ta, *maps, status, s);
-        if (err != cudaSuccess) return err;
+        if (err != cudaSuccess || plan.direct) return err;
     }
     MergeParams m;
     m.groups = plan.groups;
