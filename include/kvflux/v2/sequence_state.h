@@ -42,6 +42,10 @@ public:
     // New request sharing every page of this one (each entry retained).
     SequenceState fork_shared(RequestID new_request_id) const;
 
+    // New request sharing the first `num_blocks` pages, all of which must be
+    // full (out_of_range otherwise); it has num_blocks * block_size() tokens.
+    SequenceState fork_prefix(RequestID new_request_id, std::size_t num_blocks) const;
+
     using BlockCopier = std::function<void(PhysicalBlockHandle source,
                                            PhysicalBlockHandle destination)>;
     // Decode append with copy-on-write of a shared partial last page.

@@ -67,6 +67,14 @@ SequenceState SequenceState::fork_shared(RequestID new_request_id) const {
     return child;
 }
 
+SequenceState SequenceState::fork_prefix(RequestID new_request_id, std::size_t num_blocks) const {
+    if (num_blocks > num_tokens_ / block_size_) throw std::out_of_range("prefix beyond the sequence's full pages");
+    SequenceState child(new_request_id, table_.pool());
+    for (std::size_t i = 0; i < num_blocks; ++i) child.table_.append_shared(table_, i);
+    child.num_tokens_ = num_blocks * block_size_;
+    return child;
+}
+
 TokenLocation SequenceState::append_token_with_copy(const BlockCopier& copy) {
     if (num_tokens_ == std::numeric_limits<std::size_t>::max()) {
         throw std::overflow_error("sequence token count would overflow");

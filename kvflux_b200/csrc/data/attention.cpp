@@ -8,6 +8,7 @@
 #include "kvflux/v2/batch_block_table.h"
 #include "kvflux/v2/paged_attention.h"
 #include "kvflux/v2/paged_kv_read.h"
+#include "kvflux/v2/shared_prefix.h"
 #include "runtime.h"
 
 namespace kvflux::v2 {
@@ -173,10 +174,42 @@ void* pinned_device_address(const void* p, const char* name) {
     return a.devicePointer;
 }
 
-// Shared body of paged_attention_batch (device Q/O) and
-// paged_attention_batch_host (page-locked host Q/O).
+// kvfx_decode_shared over a batch whose table and lengths are on the device,
+// up to KVFX_MAX_PREFIX_GROUPS groups a launch.
+void decode_shared(detail::StorageRuntime& rt, const std::vector<const SequenceState*>& sequences,
+                   const std::vector<std::size_t>& lens, const detail::ResidentTable::View& table, const float* q,
+                   float* o, uint32_t query_heads, std::size_t row_elems) {
+    const std::vector<PrefixGroup> plan = plan_shared_prefixes(sequences);
+    std::size_t row = 0;
+    for (std::size_t g0 = 0; g0 < plan.size(); g0 += KVFX_MAX_PREFIX_GROUPS) {
+        kvfx_prefix_group groups[KVFX_MAX_PREFIX_GROUPS];
+        const std::size_t n = std::min<std::size_t>(KVFX_MAX_PREFIX_GROUPS, plan.size() - g0);
+        std::size_t rows = 0;
+        for (std::size_t g = 0; g < n; ++g) {
+            groups[g] = {plan[g0 + g].rows, plan[g0 + g].prefix_tokens};
+            rows += plan[g0 + g].rows;
+        }
+        const std::size_t longest = *std::max_element(lens.begin() + row, lens.begin() + row + rows);
+        const std::size_t bytes =
+            kvfx_decode_shared_workspace_bytes(&rt.cache, groups, static_cast<uint32_t>(n), query_heads, longest);
+        void* ws = rt.ensure_pieces(bytes);
+        detail::check_kvfx(kvfx_decode_shared(&rt.cache, q + row * row_elems, o + row * row_elems,
+                                              table.table + row * table.width, table.lens + row, groups,
+                                              static_cast<uint32_t>(n), table.width, query_heads, longest, ws,
+                                              rt.pieces_bytes, nullptr),
+                           "shared-prefix attention batch");
+        row += rows;
+    }
+}
+
+enum class BatchMode { kDevice, kHostIo, kShared };
+
+// Shared body of paged_attention_batch (device Q/O),
+// paged_attention_batch_host (page-locked host Q/O) and
+// paged_attention_batch_shared.
 void batch_decode(const PagedKVStorage& storage, const std::vector<const SequenceState*>& sequences,
-                  const float* query_device, float* output_device, std::size_t query_heads, bool host_io) {
+                  const float* query_device, float* output_device, std::size_t query_heads, BatchMode mode) {
+    const bool host_io = mode == BatchMode::kHostIo;
     const PagedKVLayout& layout = storage.layout();
     if (query_heads == 0 || query_heads % layout.num_kv_heads() != 0) {
         throw std::invalid_argument("invalid batch attention head count");
@@ -265,6 +298,11 @@ void batch_decode(const PagedKVStorage& storage, const std::vector<const Sequenc
     std::size_t total = 0;
     for (const std::size_t l : lens) total += l;
     const uint32_t qh = static_cast<uint32_t>(query_heads);
+    if (mode == BatchMode::kShared) {
+        decode_shared(rt, sequences, lens, table, query_device, output_device, qh, query_heads * layout.head_size());
+        rt.finish("shared-prefix attention batch synchronize");
+        return;
+    }
     // One split size for the whole batch, so that every row is computed
     // exactly as by one launch over all rows.
     const uint32_t pps = kvfx_decode_pages_per_split(&rt.cache, batch, qh, max_len, total);
@@ -332,12 +370,17 @@ void batch_decode(const PagedKVStorage& storage, const std::vector<const Sequenc
 
 void paged_attention_batch(const PagedKVStorage& storage, const std::vector<const SequenceState*>& sequences,
                            const float* query_device, float* output_device, std::size_t query_heads) {
-    batch_decode(storage, sequences, query_device, output_device, query_heads, false);
+    batch_decode(storage, sequences, query_device, output_device, query_heads, BatchMode::kDevice);
+}
+
+void paged_attention_batch_shared(const PagedKVStorage& storage, const std::vector<const SequenceState*>& sequences,
+                                  const float* query_device, float* output_device, std::size_t query_heads) {
+    batch_decode(storage, sequences, query_device, output_device, query_heads, BatchMode::kShared);
 }
 
 void paged_attention_batch_host(const PagedKVStorage& storage, const std::vector<const SequenceState*>& sequences,
                                 const float* query_host, float* output_host, std::size_t query_heads) {
-    batch_decode(storage, sequences, query_host, output_host, query_heads, true);
+    batch_decode(storage, sequences, query_host, output_host, query_heads, BatchMode::kHostIo);
 }
 
 std::size_t paged_attention_batch_table_upload_bytes(const PagedKVStorage& storage) {

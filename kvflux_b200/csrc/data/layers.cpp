@@ -7,9 +7,8 @@
 
 namespace kvflux::v2 {
 
-namespace {
+namespace detail {
 
-// Every layer non-null and of the first layer's layout and device.
 const PagedKVStorage& check_layers(const PagedKVStorage* const* layers, std::size_t n, const char* op) {
     if (n == 0) throw std::invalid_argument(std::string(op) + " needs at least one layer");
     if (n > KVFX_MAX_LAYERS) throw std::invalid_argument(std::string(op) + ": more than 128 layers");
@@ -29,36 +28,24 @@ const PagedKVStorage& check_layers(const PagedKVStorage* const* layers, std::siz
     return first;
 }
 
-std::vector<kvfx_cache> descriptors(const PagedKVStorage* const* layers, std::size_t n) {
+std::vector<kvfx_cache> layer_descriptors(const PagedKVStorage* const* layers, std::size_t n) {
     std::vector<kvfx_cache> out(n);
     for (std::size_t l = 0; l < n; ++l) out[l] = layers[l]->runtime().cache;
     return out;
 }
 
-} // namespace
-
-void write_paged_kv_layers(const std::vector<PagedKVStorage*>& layers, const void* key_new_device,
-                           const void* value_new_device, const SlotMapping& slot_mapping) {
-    std::vector<const PagedKVStorage*> view(layers.begin(), layers.end());
-    const PagedKVStorage& first = check_layers(view.data(), view.size(), "layered KV write");
-    if (slot_mapping.empty()) return;
-    if (key_new_device == nullptr || value_new_device == nullptr) {
-        throw std::invalid_argument("K_new and V_new device pointers are required");
-    }
-    const PagedKVLayout& layout = first.layout();
-    detail::StorageRuntime& rt = first.runtime();
-
-    // Range and duplicate checks in input order, as write_paged_kv.
+void check_slots(StorageRuntime& rt, const PagedKVLayout& layout, const SlotMapping& slots) {
+    // One bit per slot, cleared after.
     const std::size_t words = (layout.slot_count() + 63) / 64;
     if (rt.seen.size() < words) rt.seen.assign(words, 0);
     std::size_t checked = 0;
     auto clear_seen = [&] {
         for (std::size_t i = 0; i < checked; ++i) {
-            const PhysicalSlot s = slot_mapping[i];
+            const PhysicalSlot s = slots[i];
             rt.seen[s >> 6] &= ~(std::uint64_t{1} << (s & 63));
         }
     };
-    for (const PhysicalSlot s : slot_mapping) {
+    for (const PhysicalSlot s : slots) {
         if (s >= layout.slot_count()) {
             clear_seen();
             throw std::out_of_range("KV write slot out of range");
@@ -73,6 +60,22 @@ void write_paged_kv_layers(const std::vector<PagedKVStorage*>& layers, const voi
         ++checked;
     }
     clear_seen();
+}
+
+} // namespace detail
+
+void write_paged_kv_layers(const std::vector<PagedKVStorage*>& layers, const void* key_new_device,
+                           const void* value_new_device, const SlotMapping& slot_mapping) {
+    std::vector<const PagedKVStorage*> view(layers.begin(), layers.end());
+    const PagedKVStorage& first = detail::check_layers(view.data(), view.size(), "layered KV write");
+    if (slot_mapping.empty()) return;
+    if (key_new_device == nullptr || value_new_device == nullptr) {
+        throw std::invalid_argument("K_new and V_new device pointers are required");
+    }
+    const PagedKVLayout& layout = first.layout();
+    detail::StorageRuntime& rt = first.runtime();
+
+    detail::check_slots(rt, layout, slot_mapping);  // in input order, as write_paged_kv
 
     const std::size_t elements = detail::mul_checked(
         detail::mul_checked(slot_mapping.size(), layout.num_kv_heads(), "layered KV write"), layout.head_size(),
@@ -87,7 +90,7 @@ void write_paged_kv_layers(const std::vector<PagedKVStorage*>& layers, const voi
     const void* host[1] = {slot_mapping.data()};
     void* dev[1] = {nullptr};
     rt.upload(host, &slot_bytes, 1, dev);
-    const std::vector<kvfx_cache> caches = descriptors(view.data(), view.size());
+    const std::vector<kvfx_cache> caches = detail::layer_descriptors(view.data(), view.size());
     detail::check_kvfx(kvfx_write_layers(caches.data(), static_cast<uint32_t>(caches.size()), key_new_device,
                                          value_new_device, layer_bytes, static_cast<const uint64_t*>(dev[0]),
                                          slot_mapping.size(), nullptr),
@@ -97,7 +100,7 @@ void write_paged_kv_layers(const std::vector<PagedKVStorage*>& layers, const voi
 
 void read_paged_kv_layers(const std::vector<const PagedKVStorage*>& layers, const SequenceState& sequence,
                           void* key_out_device, void* value_out_device) {
-    const PagedKVStorage& first = check_layers(layers.data(), layers.size(), "layered KV read");
+    const PagedKVStorage& first = detail::check_layers(layers.data(), layers.size(), "layered KV read");
     for (const PagedKVStorage* l : layers) {
         if (!l->uses_pool(sequence.block_table())) {
             throw std::invalid_argument("sequence and KV storage must use one physical pool");
@@ -142,7 +145,7 @@ void read_paged_kv_layers(const std::vector<const PagedKVStorage*>& layers, cons
     void* dev[4] = {nullptr, nullptr, nullptr, nullptr};
     detail::StorageRuntime& rt = first.runtime();
     rt.upload(host, bytes, 4, dev);
-    const std::vector<kvfx_cache> caches = descriptors(layers.data(), layers.size());
+    const std::vector<kvfx_cache> caches = detail::layer_descriptors(layers.data(), layers.size());
     detail::check_kvfx(kvfx_gather_layers(caches.data(), static_cast<uint32_t>(caches.size()),
                                           static_cast<const uint64_t*>(dev[0]), static_cast<const uint64_t*>(dev[1]),
                                           1, blocks.size(), static_cast<void* const*>(dev[2]),

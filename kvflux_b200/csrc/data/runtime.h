@@ -45,6 +45,17 @@ private:
 void require_device_pointer(const void* p, int device, const char* name);
 bool overlaps(const void* a, std::size_t a_bytes, const void* b, std::size_t b_bytes);
 
+// The checks every layered call makes: at least one layer, at most
+// KVFX_MAX_LAYERS, none null, all of the first one's layout and device.
+// Returns the first.
+const PagedKVStorage& check_layers(const PagedKVStorage* const* layers, std::size_t n, const char* op);
+std::vector<kvfx_cache> layer_descriptors(const PagedKVStorage* const* layers, std::size_t n);
+
+struct StorageRuntime;
+// out_of_range for a slot beyond the layout, invalid_argument for one that
+// appears twice, whichever comes first in the mapping.
+void check_slots(StorageRuntime& rt, const PagedKVLayout& layout, const SlotMapping& slots);
+
 // One run of a table patch: ids[src, src + count) go to table[dst, dst + count).
 struct TablePatchRun {
     uint64_t dst;
@@ -54,8 +65,6 @@ struct TablePatchRun {
 // Enqueues the copy of every run (table, runs and ids are device memory).
 cudaError_t launch_table_patch(uint64_t* table, const TablePatchRun* runs, const uint64_t* ids, uint32_t num_runs,
                                cudaStream_t stream);
-
-struct StorageRuntime;
 
 // The device-resident copy of the padded [rows][width] page table of the last
 // batch decode on a storage (reference: build_batch_block_table,
@@ -167,6 +176,11 @@ struct StorageRuntime {
     void* io = nullptr;
     std::size_t io_bytes = 0;
     void* ensure_io(std::size_t bytes);
+    // Scratch of kvfx_decode_shared (holds nothing between calls; the decode
+    // workspaces' counters must stay zero, so it has its own).
+    void* pieces = nullptr;
+    std::size_t pieces_bytes = 0;
+    void* ensure_pieces(std::size_t bytes);
     // Synchronises the legacy default stream and raises on device-side flags.
     void finish(const char* op) const;
     // Device-resident page table of paged_attention_batch(_host), and the

@@ -61,6 +61,7 @@ StorageRuntime::~StorageRuntime() {
     if (workspace) (void)cudaFree(workspace);
     if (workspace2) (void)cudaFree(workspace2);
     if (io) (void)cudaFree(io);
+    if (pieces) (void)cudaFree(pieces);
     if (pinned) (void)cudaFreeHost(pinned);
     if (side_ready) (void)cudaEventDestroy(side_ready);
     if (side_done) (void)cudaEventDestroy(side_done);
@@ -156,6 +157,17 @@ void* StorageRuntime::ensure_io(std::size_t bytes) {
         io_bytes = bytes;
     }
     return io;
+}
+
+void* StorageRuntime::ensure_pieces(std::size_t bytes) {
+    if (bytes > pieces_bytes) {
+        if (pieces) cuda_check(cudaFree(pieces), "free workspace");
+        pieces = nullptr;
+        pieces_bytes = 0;
+        cuda_check(cudaMalloc(&pieces, bytes), "allocate workspace");
+        pieces_bytes = bytes;
+    }
+    return pieces;
 }
 
 void StorageRuntime::finish(const char* op) const {

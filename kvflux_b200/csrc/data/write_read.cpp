@@ -18,31 +18,8 @@ void write_paged_kv(PagedKVStorage& storage, const void* key_new_device, const v
     detail::StorageRuntime& rt = storage.runtime();
 
     // Range and duplicate checks in input order (the first offence decides the
-    // exception type, as in the reference). One bit per slot, cleared after.
-    const std::size_t words = (layout.slot_count() + 63) / 64;
-    if (rt.seen.size() < words) rt.seen.assign(words, 0);
-    std::size_t checked = 0;
-    auto clear_seen = [&] {
-        for (std::size_t i = 0; i < checked; ++i) {
-            const PhysicalSlot s = slot_mapping[i];
-            rt.seen[s >> 6] &= ~(std::uint64_t{1} << (s & 63));
-        }
-    };
-    for (const PhysicalSlot s : slot_mapping) {
-        if (s >= layout.slot_count()) {
-            clear_seen();
-            throw std::out_of_range("KV write slot out of range");
-        }
-        std::uint64_t& w = rt.seen[s >> 6];
-        const std::uint64_t bit = std::uint64_t{1} << (s & 63);
-        if (w & bit) {
-            clear_seen();
-            throw std::invalid_argument("duplicate KV write slot");
-        }
-        w |= bit;
-        ++checked;
-    }
-    clear_seen();
+    // exception type, as in the reference).
+    detail::check_slots(rt, layout, slot_mapping);
 
     const std::size_t elements = detail::mul_checked(
         detail::mul_checked(slot_mapping.size(), layout.num_kv_heads(), "paged KV write"),

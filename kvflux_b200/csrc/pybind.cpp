@@ -12,13 +12,16 @@
 #include "kvflux/v2/batch_decode_session.h"
 #include "kvflux/v2/copy_on_write.h"
 #include "kvflux/v2/paged_attention.h"
+#include "kvflux/v2/paged_kv_fork.h"
 #include "kvflux/v2/paged_kv_layers.h"
 #include "kvflux/v2/paged_kv_read.h"
 #include "kvflux/v2/paged_kv_storage.h"
 #include "kvflux/v2/paged_kv_write.h"
 #include "kvflux/v2/prefix_cache.h"
 #include "kvflux/v2/reference_attention.h"
+#include "kvflux/v2/rotary.h"
 #include "kvflux/v2/sequence_lifecycle.h"
+#include "kvflux/v2/shared_prefix.h"
 #include "kvflux/v2/slot_mapping.h"
 
 namespace py = pybind11;
@@ -161,6 +164,7 @@ PYBIND11_MODULE(_C, m) {
         .def("append_tokens", &SequenceState::append_tokens)
         .def("append_token", &SequenceState::append_token)
         .def("fork_shared", &SequenceState::fork_shared, py::keep_alive<0, 1>())
+        .def("fork_prefix", &SequenceState::fork_prefix, py::keep_alive<0, 1>())
         .def("append_token_with_copy",
              [](SequenceState& s, py::object copier) {
                  if (copier.is_none()) return s.append_token_with_copy({});
@@ -262,6 +266,51 @@ PYBIND11_MODULE(_C, m) {
               paged_attention_prefill_batch(s, seqs, q, o, query_tokens, query_heads);
           });
     m.def("append_token_cow", &append_token_cow);
+    py::class_<PrefixGroup>(m, "PrefixGroup")
+        .def_readonly("rows", &PrefixGroup::rows)
+        .def_readonly("prefix_tokens", &PrefixGroup::prefix_tokens);
+    m.def("plan_shared_prefixes", &plan_shared_prefixes);
+    m.def("paged_attention_batch_shared",
+          [](const PagedKVStorage& s, const std::vector<const SequenceState*>& seqs, py::object q, py::object o,
+             std::size_t query_heads) {
+              paged_attention_batch_shared(s, seqs, ptr<const float>(q), ptr<float>(o), query_heads);
+          });
+    m.def("fork_sequence", [](const std::vector<PagedKVStorage*>& layers, py::object source,
+                              const std::vector<RequestID>& children) {
+        std::vector<SequenceState> made = fork_sequence(layers, source.cast<const SequenceState&>(), children);
+        py::list out;
+        for (SequenceState& child : made) {
+            py::object o = py::cast(std::move(child));
+            py::detail::keep_alive_impl(o, source);  // the pool stays alive, as for fork_shared
+            out.append(o);
+        }
+        return out;
+    });
+    m.def("compact_sequence", &compact_sequence);
+    py::class_<RotaryTable>(m, "RotaryTable")
+        .def(py::init<std::size_t, std::size_t, double, double, bool, int>(), py::arg("max_positions"),
+             py::arg("rotary_dim"), py::arg("base") = 10000.0, py::arg("position_scale") = 1.0,
+             py::arg("interleaved") = false, py::arg("device") = 0)
+        .def("max_positions", &RotaryTable::max_positions)
+        .def("rotary_dim", &RotaryTable::rotary_dim)
+        .def("interleaved", &RotaryTable::interleaved)
+        .def("device", &RotaryTable::device)
+        .def("device_table", [](const RotaryTable& t) { return reinterpret_cast<std::uintptr_t>(t.device_table()); });
+    m.def(
+        "write_paged_kv_rotated",
+        [](PagedKVStorage& s, const RotaryTable& table, py::object q, py::object k, py::object v,
+           std::size_t query_stride, std::size_t key_stride, std::size_t value_stride, std::size_t query_heads,
+           const std::vector<std::size_t>& positions, const SlotMapping& slots, py::object q_out,
+           py::object query_weight, py::object key_weight, float epsilon) {
+            write_paged_kv_rotated(s, table, {ptr<const float>(query_weight), ptr<const float>(key_weight), epsilon},
+                                   {ptr<const void>(q), ptr<const void>(k), ptr<const void>(v), query_stride,
+                                    key_stride, value_stride},
+                                   query_heads, positions, slots, ptr<float>(q_out));
+        },
+        py::arg("storage"), py::arg("table"), py::arg("query"), py::arg("key"), py::arg("value"),
+        py::arg("query_stride"), py::arg("key_stride"), py::arg("value_stride"), py::arg("query_heads"),
+        py::arg("positions"), py::arg("slots"), py::arg("query_out"), py::arg("query_weight") = py::none(),
+        py::arg("key_weight") = py::none(), py::arg("epsilon") = 1e-6f);
     m.def("write_paged_kv_layers", [](const std::vector<PagedKVStorage*>& layers, py::object k, py::object v,
                                       const SlotMapping& slots) {
         write_paged_kv_layers(layers, ptr<const void>(k), ptr<const void>(v), slots);
