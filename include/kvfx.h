@@ -50,7 +50,7 @@ extern "C" {
 #define KVFX_MAX_PREFILL_SEQS 32u
 
 /* Most groups one kvfx_decode_shared call takes. */
-#define KVFX_MAX_PREFIX_GROUPS 128u
+#define KVFX_MAX_PREFIX_GROUPS 32u
 
 /* Slot of a padding token (kvfx_write_rotated): nothing is written for it. */
 #define KVFX_NO_SLOT UINT64_MAX

@@ -37,7 +37,7 @@ KVFX_F16, KVFX_BF16, KVFX_F32 = 0, 1, 2
 KVFX_FLAG_BAD_INDEX, KVFX_FLAG_TIMEOUT = 1, 2
 KVFX_MAX_LAYERS = 128
 KVFX_MAX_PREFILL_SEQS = 32
-KVFX_MAX_PREFIX_GROUPS = 128
+KVFX_MAX_PREFIX_GROUPS = 32
 KVFX_NO_SLOT = 2**64 - 1
 
 

@@ -38,12 +38,14 @@ def clear_status(cuda):
 class Batch:
     """Rows on a permuted pool whose unwritten slots hold NaN."""
 
-    def __init__(self, groups, lens, heads, group, hd, bs=16, dtype="bfloat16", seed=1, q_scale=1.0, k_drift=0.0):
+    def __init__(self, groups, lens, heads, group, hd, bs=16, dtype="bfloat16", seed=1, q_scale=1.0, k_drift=0.0, room=0):
         self.groups, self.lens, self.heads, self.hq, self.hd, self.bs, self.dtype = groups, lens, heads, heads * group, hd, bs, dtype
         gen = torch.Generator().manual_seed(seed)
         rows = [g for g, (n, _) in enumerate(groups) for _ in range(n)]
         assert len(rows) == len(lens)
-        self.max_len = max(max(lens), max(p for _, p in groups))
+        # `room`: the host's bound above the longest row. Past 640 tokens the groups' prefixes are shared by the
+        # tensor-core kernel; below, one launch reads row by row (as long as the rows fit one wave).
+        self.max_len = max(max(lens), max(p for _, p in groups)) + room
         self.width = -(-self.max_len // bs) + 2
         self.table = np.full((len(rows), self.width), 2**64 - 1, np.uint64)
         need = sum(p // bs for _, p in groups) + sum(max(0, -(-n // bs) - groups[g][1] // bs) for g, n in zip(rows, lens))
@@ -122,7 +124,7 @@ CASES = [  # groups (rows, prefix), lens, heads, q_group, hd, bs, dtype
     ([(64, 256)], [256 + i for i in range(64)], 1, 4, 64, 16, "bfloat16"),                     # exactly two query tiles
     ([(3, 48), (2, 320)], [48, 49, 100, 321, 999], 2, 12, 128, 16, "float16"),                 # q_group above 8
     ([(9, 128 * 37)], [128 * 37 + 1] * 9, 1, 7, 128, 16, "bfloat16"),                          # one pair over many CTAs
-    ([(2, 16 * (1 + g % 11)) for g in range(128)], [16 * (1 + g // 2 % 11) + g % 5 for g in range(256)], 2, 2, 64, 16, "bfloat16"),
+    ([(2, 16 * (1 + g % 11)) for g in range(32)], [16 * (1 + g // 2 % 11) + g % 5 for g in range(64)], 2, 2, 64, 16, "bfloat16"),
     ([(4, 256), (3, 160)], [0, 256, 300, 0, 0, 0, 0], 2, 4, 128, 16, "bfloat16"),              # padding rows, a group of nothing else
     ([(3, 0)], [1, 33, 700], 2, 4, 128, 16, "bfloat16"),                                       # nothing shared
     ([(3, 64), (2, 0)], [64, 70, 0, 5, 129], 2, 2, 32, 8, "float32"),                          # row by row
@@ -131,9 +133,10 @@ CASES = [  # groups (rows, prefix), lens, heads, q_group, hd, bs, dtype
 ]
 
 
+@pytest.mark.parametrize("room", [0, 1000])
 @pytest.mark.parametrize("groups,lens,heads,group,hd,bs,dtype", CASES)
-def test_against_every_row_alone(groups, lens, heads, group, hd, bs, dtype):
-    b = Batch(groups, lens, heads, group, hd, bs, dtype)
+def test_against_every_row_alone(groups, lens, heads, group, hd, bs, dtype, room):
+    b = Batch(groups, lens, heads, group, hd, bs, dtype, room=room)
     got = b.run()
     assert kv.device_status(0) == 0
     b.check(got)
@@ -150,9 +153,10 @@ def test_large_and_growing_scores(dtype, hd):
     assert kv.device_status(0) == 0
 
 
-def test_rows_outside_their_bounds_are_refused():
-    b = Batch([(4, 256)], [256, 300, 400, 290], 2, 4, 128)
-    lens = [255, 300, 401, 240]
+@pytest.mark.parametrize("room", [0, 1000])
+def test_rows_outside_their_bounds_are_refused(room):
+    b = Batch([(4, 256)], [256, 300, 400, 290], 2, 4, 128, room=room)
+    lens = [255, 300, 401 + room, 240]
     b.dlens = u64(np.array(lens, np.uint64))
     got = b.run()
     assert kv.device_status(0) == kv.KVFX_FLAG_BAD_INDEX
@@ -165,10 +169,11 @@ def test_rows_outside_their_bounds_are_refused():
     assert torch.all(got[1] == 7.0)
 
 
+@pytest.mark.parametrize("room", [0, 1000])
 @pytest.mark.parametrize("row,col", [(0, 3), (1, 17)])
-def test_bad_pages_are_flagged(row, col):
+def test_bad_pages_are_flagged(row, col, room):
     """A prefix page (of the group's first row) or a row's own page outside the pool."""
-    b = Batch([(2, 256)], [300, 300], 2, 4, 128)
+    b = Batch([(2, 256)], [300, 300], 2, 4, 128, room=room)
     table = b.table.copy()
     table[row, col] = b.pages
     b.dtable = u64(table)
@@ -178,8 +183,9 @@ def test_bad_pages_are_flagged(row, col):
         b.check(got, rows=[0])
 
 
-def test_only_the_first_row_names_the_prefix():
-    b = Batch([(3, 256)], [300, 270, 256], 2, 4, 128)
+@pytest.mark.parametrize("room", [0, 1000])
+def test_only_the_first_row_names_the_prefix(room):
+    b = Batch([(3, 256)], [300, 270, 256], 2, 4, 128, room=room)
     table = b.table.copy()
     table[1:, :16] = b.pages + 5
     b.dtable = u64(table)
@@ -187,8 +193,9 @@ def test_only_the_first_row_names_the_prefix():
     assert kv.device_status(0) == 0
 
 
-def test_replayed_graph_reads_the_lengths_of_the_day():
-    b = Batch([(3, 256), (2, 32)], [300, 400, 256, 40, 33], 2, 4, 128)
+@pytest.mark.parametrize("room", [0, 1000])
+def test_replayed_graph_reads_the_lengths_of_the_day(room):
+    b = Batch([(3, 256), (2, 32)], [300, 400, 256, 40, 33], 2, 4, 128, room=room)
     out = torch.full((5, b.hq, b.hd), 7.0, device="cuda")
     side, graph = torch.cuda.Stream(), torch.cuda.CUDAGraph()
     torch.cuda.synchronize()
@@ -220,8 +227,9 @@ def test_two_streams_with_workspaces_of_their_own():
     assert kv.device_status(0) == 0
 
 
-def test_agrees_with_the_plain_decode():
-    b = Batch([(6, 512)], [520 + 3 * i for i in range(6)], 2, 4, 128)
+@pytest.mark.parametrize("room", [0, 1000])
+def test_agrees_with_the_plain_decode(room):
+    b = Batch([(6, 512)], [520 + 3 * i for i in range(6)], 2, 4, 128, room=room)
     got = b.run()
     need = kv.lib.kvfx_decode_workspace_bytes(ctypes.byref(b.cache), 6, b.hq, b.max_len, 0)
     ws = torch.zeros(need, dtype=torch.uint8, device="cuda")
@@ -229,3 +237,36 @@ def test_agrees_with_the_plain_decode():
     call(kv.lib.kvfx_decode, ctypes.byref(b.cache), b.dq, out, b.dtable, b.dlens, 6, b.width, b.hq, b.max_len, 0, ws, need, None)
     b.check(out.cpu())
     b.check(got)
+
+
+def test_captured_forks_beside_an_eager_call():
+    """A capture on one stream while another stream's eager call uses a workspace of its own."""
+    a = Batch([(4, 1040)], [1040, 1100, 1300, 1041], 2, 4, 64, seed=5)
+    b = Batch([(4, 1040)], [1040, 1100, 1300, 1041], 2, 4, 64, seed=6)
+    outs = [torch.full((4, 8, 64), 7.0, device="cuda") for _ in range(2)]
+    side, other, graph = torch.cuda.Stream(), torch.cuda.Stream(), torch.cuda.CUDAGraph()
+    torch.cuda.synchronize()
+    with torch.cuda.graph(graph, stream=side, capture_error_mode="thread_local"):
+        kv.check(kv.lib.kvfx_decode_shared(*a.args(outs[0], stream=side.cuda_stream)), "capture")
+    graph.replay()
+    kv.check(kv.lib.kvfx_decode_shared(*b.args(outs[1], stream=other.cuda_stream)), "eager")
+    graph.replay()
+    torch.cuda.synchronize()
+    a.check(outs[0].cpu())
+    b.check(outs[1].cpu())
+
+
+def test_lengths_rows_and_heads_at_random():
+    """Seeded shapes over the whole range: groups, rows, prefixes, own tokens, heads, types."""
+    rng = np.random.default_rng(7)
+    for i in range(24):
+        heads, group = int(rng.choice([1, 2, 3])), int(rng.choice([1, 2, 3, 5, 8, 12]))
+        groups = [(int(rng.integers(1, 40 // (g + 1) + 1)), int(rng.integers(0, 90)) * 16) for g in range(int(rng.integers(1, 5)))]
+        lens = [p + int(rng.choice([0, 1, 15, 16, 17, int(rng.integers(1, 400))])) for n, p in groups for _ in range(n)]
+        lens = [n if rng.random() > 0.1 else 0 for n in lens]
+        if not any(lens):
+            lens[0] = groups[0][1] + 1
+        b = Batch(groups, lens, heads, group, int(rng.choice([64, 128])), dtype=str(rng.choice(["float16", "bfloat16"])), seed=100 + i,
+                  room=int(rng.choice([0, 1000])))
+        b.check(b.run())
+        assert kv.device_status(0) == 0

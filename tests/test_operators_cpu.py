@@ -67,7 +67,7 @@ def test_shared_decode_refuses_bad_arguments():
     assert kv.lib.kvfx_decode_shared(None, 1, 1, 1, 1, None, 0, 4, 4, 64, None, 0, None) == kv.KVFX_EINVAL
     assert f(groups=(), q=None, o=None, table=None, lens=None) == kv.KVFX_OK
     for bad in (dict(hq=3), dict(hq=0), dict(groups=None, n=1), dict(groups=((0, 32),)), dict(groups=((2, 33),)), dict(groups=((2, 80),)),
-                dict(groups=((65535, 0), (1, 0))), dict(groups=((2**63, 0), (2**63, 0))), dict(groups=((1, 0),) * 129), dict(q=None), dict(o=None),
+                dict(groups=((65535, 0), (1, 0))), dict(groups=((2**63, 0), (2**63, 0))), dict(groups=((1, 0),) * 33), dict(q=None), dict(o=None),
                 dict(table=None), dict(lens=None), dict(width=3), dict(max_len=0)):
         assert f(**bad) == kv.KVFX_EINVAL, bad
     fast = _cache(num_blocks=1024, num_kv_heads=8, head_size=128)
