@@ -17,12 +17,15 @@
 //   warp 0, 2   K and V producers: per tile up to 8 pages, one tensor load
 //               each (128-byte swizzle, no multicast), into rings of 2 (hd
 //               128) or 5 (hd 64) tiles. A load brings a page's 16 rows of one
-//               head as [2 groups of 8 rows][hd / 64][8 rows][128 bytes]: 4 KiB
-//               at hd 128, where a box of one 64-dim half would be 2 KiB (one
-//               thread issues about one box per 50 ns, whatever its size).
-//   warp 1      owns TMEM and issues every tcgen05.mma: S(t) = Q K_t^T with Q
-//               from TMEM, two tiles ahead of O += P(t) V_t with P from TMEM.
-//   warp 3      idle.
+//               head as [2 groups of 8 rows][hd / 64][8 rows][128 bytes]. The
+//               loads' coordinates are worked out ahead by all lanes, so that
+//               the issuing lane spends 0.3 us a tile: the rings being short,
+//               that time is part of a tile's (1.75 us with 1.5 us of it, 1.45
+//               now).
+//   warp 1      owns TMEM and issues S(t) = Q K_t^T, Q from TMEM, once PV(t - 2)
+//               has read P(t - 2), which lies in the same columns.
+//   warp 3      issues O += P(t) V_t, P from TMEM. (One warp issuing both
+//               groups in turn spends 0.6 us of a tile's time between them.)
 //   warps 4-7   softmax, one query row per thread (TMEM lane = row): row
 //               maximum, then P = 2^(S - m) over its own S columns as packed
 //               hi/lo pairs.
@@ -31,8 +34,6 @@
 //               from zero again), and store a finished segment's sum.
 // Warps all of whose query rows lie past the tile's last one only signal.
 // TMEM columns: S/P buffers 0 and 128; O 256; Q behind it (hi then lo halves).
-// S[t % 2] holds P(t) until PV(t) has read it; QK(t + 2) is issued after PV(t)
-// by the same thread, and one thread's MMAs execute in order.
 // Precision: Q and P are fed as two 16-bit operands each, hi = round(x) and
 // lo = round(x - hi): about 16 mantissa bits (one 16-bit operand alone is off
 // by 2^-9 of each weight). The tensor cores truncate each sum into the FP32
@@ -41,7 +42,10 @@
 // which rounds. (Kept in registers it is code that runs out of a cold
 // instruction cache at every segment's end, 6 us more at 7 tiles a CTA; left
 // to the merge kernel, 16 tiles a piece, it is 60 MB more to write and read at
-// 256 rows x 64 heads.) O is rescaled in TMEM only when a tile's row maximum
+// 256 rows x 64 heads.) A flush takes all of O into registers and lets the
+// next PV go before it adds: 208 us against 218 at 256 rows x 64 heads x 16384
+// tokens, 620 -> 660 TFLOP/s of attention (twice that executed), where a tile
+// is bounded by its chain: softmax 1.2 us, PV and QK 0.6 us each. O is rescaled in TMEM only when a tile's row maximum
 // passes the running one by more than 8.
 #include <algorithm>
 #include <atomic>
@@ -182,42 +186,50 @@ __device__ __noinline__ void produce(const PrefixParams& p, const CUtensorMap* m
         return __all_sync(0xffffffffu, mbar_wait_lean(bar, phase, p.status)) != 0;
     };
     pdl_wait();
-    // Page ids, four tiles (32 pages, one a lane) at a time and the next four
-    // fetched behind them, so that a table read's latency is never waited for
-    // but at a segment's start.
+    // Where the pages are (in groups of 8 rows, counted through the cache's
+    // pages and heads), four tiles (32 pages, one a lane) at a time and the
+    // next four fetched behind them, so that a table read's latency is never
+    // waited for but at a segment's start.
     const uint64_t* row = nullptr;
     uint32_t pages = 0, kh = 0;
     auto fetch = [&](uint32_t page0) -> uint64_t { return page0 + lane < pages ? __ldg(row + page0 + lane) : 0; };
+    auto place = [&](uint64_t id) -> int {
+        if (id >= p.num_blocks) {
+            raise_flag(p.status, KVFX_FLAG_BAD_INDEX);
+            id = 0;
+        }
+        return static_cast<int>((id * p.kv_heads + kh) * 2);
+    };
     // Streamed through the L2, but for groups of several query tiles, which
     // read each page once a tile.
     const uint64_t policy = p.stream ? l2_evict_first() : l2_evict_normal();
-    uint64_t ids = 0, ids_next = 0;
+    int at = 0;
+    uint64_t ids_next = 0;
     uint32_t issued = 0;
     for (; c.valid(); c.step()) {
         if (c.first()) {
             row = p.table + static_cast<uint64_t>(c.list[c.k].row0) * p.max_blocks;
             pages = c.pages;
             kh = c.list[c.k].kh;
-            ids = fetch(c.j / 4 * 32);
+            at = place(fetch(c.j / 4 * 32));
             ids_next = fetch(c.j / 4 * 32 + 32);
         } else if (c.j % 4 == 0) {
-            ids = ids_next;
+            at = place(ids_next);
             ids_next = fetch((c.j / 4 + 1) * 32);
         }
+        int tile_at[kTilePages];
+#pragma unroll
+        for (int pg = 0; pg < kTilePages; ++pg) tile_at[pg] = __shfl_sync(0xffffffffu, at, c.j % 4 * 8 + pg);
         const uint32_t st = c.t % S::kStages;
         if (c.t >= S::kStages && !wait(&freed[st], (c.t / S::kStages - 1) & 1u)) break;
         const uint32_t n = c.tile_pages();
-        if (leader) mbar_arrive_expect_tx(&full[st], n * S::kPage);
-        for (uint32_t pg = 0; pg < n; ++pg) {
-            uint64_t blk = __shfl_sync(0xffffffffu, ids, c.j % 4 * 8 + pg);
-            if (!leader) continue;
-            if (blk >= p.num_blocks) {
-                raise_flag(p.status, KVFX_FLAG_BAD_INDEX);
-                blk = 0;
+        if (leader) {
+            mbar_arrive_expect_tx(&full[st], n * S::kPage);
+#pragma unroll
+            for (uint32_t pg = 0; pg < kTilePages; ++pg) {
+                if (pg < n)
+                    tma_load_4d_hint(ring + st * S::kTile + pg * S::kPage, map, 0, 0, 0, tile_at[pg], &full[st], policy);
             }
-            // Groups of 8 rows count through the cache's pages and heads.
-            tma_load_4d_hint(ring + st * S::kTile + pg * S::kPage, map, 0, 0, 0,
-                             static_cast<int>((blk * p.kv_heads + kh) * 2), &full[st], policy);
         }
         issued = c.t + 1;
     }
@@ -264,7 +276,7 @@ prefix_tc_kernel(const __grid_constant__ PrefixParams p, const __grid_constant__
             mbar_init(&ml_full[b], 128);
             mbar_init(&ml_free[b], 128);
         }
-        mbar_init(&mma_done, 1);
+        mbar_init(&mma_done, 2);
         fence_mbarrier_init();
     }
     if (warp == 0 && elect_one()) prefetch_tensormap(&kmap);
@@ -288,34 +300,24 @@ prefix_tc_kernel(const __grid_constant__ PrefixParams p, const __grid_constant__
         produce<HD>(p, &kmap, start, smem, k_full, k_free);
     } else if (warp == 2) {
         produce<HD>(p, &vmap, start, smem + S::kOffV, v_full, v_free);
-    } else if (warp == 3) {
-        // The next kernel may start once what lies ahead of this one is
-        // complete: the tail kernel reads Q, K, V and tables without a wait.
-        pdl_wait();
-        pdl_allow_next();
     } else if (warp == 1) {
-        // ----------------------------------------------------- MMA issuer ---
+        // ------------------------------------------------------ QK issuer ---
         // The whole warp runs the schedule; one elected lane issues.
         const bool leader = elect_one();
         auto wait = [&](uint64_t* bar, uint32_t phase) {
             return __all_sync(0xffffffffu, mbar_wait_lean(bar, phase, p.status)) != 0;
         };
-        constexpr bool kBF = std::is_same<T, __nv_bfloat16>::value;
-        const uint32_t id_qk = tc::idesc_f16(kBM, kBN, kBF, false);
-        const uint32_t id_pv = tc::idesc_f16(kBM, HD, kBF, true);
-        // K: 8-token groups kGroup apart, 64 dims to the next block 1 KiB; V
-        // (MN-major): the next 64 dims 1 KiB on, 8-token groups kGroup apart.
+        const uint32_t id_qk = tc::idesc_f16(kBM, kBN, std::is_same<T, __nv_bfloat16>::value, false);
+        // K: 8-token groups kGroup apart, 64 dims to the next block 1 KiB.
         const uint64_t k_desc0 = tc::smem_desc(sbase, 16, S::kGroup);
-        const uint64_t v_desc0 = tc::smem_desc(sbase + S::kOffV, 1024, S::kGroup);
-        Cursor qk = start, pv = start;
-        // S(t) = Q K_t^T into S[t % 2], whose P(t - 2) PV(t - 2) (issued
-        // before by this thread) reads first.
-        auto qk_step = [&]() -> bool {
-            const uint32_t st = qk.t % S::kStages;
-            if (qk.first() && !wait(&q_full, qk.k & 1u)) return false;
-            if (!wait(&k_full[st], (qk.t / S::kStages) & 1u)) return false;
+        // S(t) = Q K_t^T into S[t % 2], once PV(t - 2) has read P(t - 2) there.
+        for (Cursor c = start; c.valid(); c.step()) {
+            const uint32_t st = c.t % S::kStages, b = c.t % kSBufs;
+            if (c.first() && !wait(&q_full, c.k & 1u)) break;
+            if (!wait(&k_full[st], (c.t / S::kStages) & 1u)) break;
+            if (c.t >= kSBufs && !wait(&pv_done[b], (c.t / kSBufs - 1) & 1u)) break;
             tc::fence_after_sync();
-            const uint32_t d = tmem + (qk.t % kSBufs) * kBN;
+            const uint32_t d = tmem + b * kBN;
             const uint64_t k_desc = k_desc0 + ((st * S::kTile) >> 4);
             if (leader) {
                 // Q_hi, then Q_lo, in K-steps of 16 dims (8 columns of Q; 64
@@ -326,26 +328,39 @@ prefix_tc_kernel(const __grid_constant__ PrefixParams p, const __grid_constant__
                     tc::mma_ts(d, tmem + S::kTmemQ + i * 8, k_desc + (((kk >> 2) * 1024 + (kk & 3) * 32) >> 4), id_qk,
                                i > 0 ? 1u : 0u);
                 }
-                tc::commit(&s_full[qk.t % kSBufs]);
+                tc::commit(&s_full[b]);
                 tc::commit(&k_free[st]);
-                if (qk.last()) tc::commit(&q_free);  // Q may be replaced once this completes
+                if (c.last()) tc::commit(&q_free);  // Q may be replaced once this completes
             }
-            qk.step();
-            return true;
+        }
+        // Every MMA issued is complete before TMEM is released.
+        if (leader) tc::commit(&mma_done);
+        (void)wait(&mma_done, 0);
+    } else if (warp == 3) {
+        // ------------------------------------------------------ PV issuer ---
+        // First: the next kernel may start once what lies ahead of this one
+        // is complete (the tail kernel reads Q, K, V and tables without a wait).
+        pdl_wait();
+        pdl_allow_next();
+        const bool leader = elect_one();
+        auto wait = [&](uint64_t* bar, uint32_t phase) {
+            return __all_sync(0xffffffffu, mbar_wait_lean(bar, phase, p.status)) != 0;
         };
+        const uint32_t id_pv = tc::idesc_f16(kBM, HD, std::is_same<T, __nv_bfloat16>::value, true);
+        // V (MN-major): the next 64 dims 1 KiB on, 8-token groups kGroup apart.
+        const uint64_t v_desc0 = tc::smem_desc(sbase + S::kOffV, 1024, S::kGroup);
         // O += P(t) V_t over the tile's valid pages (16 tokens = one K-step).
         // A flush's first PV overwrites O, which must have been read.
         uint32_t flush = 0, in_flush = 0;
-        auto pv_step = [&]() -> bool {
-            const uint32_t st = pv.t % S::kStages, b = pv.t % kSBufs;
-            const bool first = in_flush == 0;
-            if (first && flush >= 1 && !wait(&o_free, (flush - 1) & 1u)) return false;
-            if (!wait(&v_full[st], (pv.t / S::kStages) & 1u)) return false;
-            if (!wait(&p_full[b], (pv.t / kSBufs) & 1u)) return false;
+        for (Cursor c = start; c.valid(); c.step()) {
+            const uint32_t st = c.t % S::kStages, b = c.t % kSBufs;
+            const bool first = in_flush == 0, last = c.last() || in_flush + 1 == kFlush;
+            if (first && flush >= 1 && !wait(&o_free, (flush - 1) & 1u)) break;
+            if (!wait(&v_full[st], (c.t / S::kStages) & 1u)) break;
+            if (!wait(&p_full[b], (c.t / kSBufs) & 1u)) break;
             tc::fence_after_sync();
-            const uint32_t pt = tmem + b * kBN, n = pv.tile_pages();
+            const uint32_t pt = tmem + b * kBN, n = c.tile_pages();
             const uint64_t v_desc = v_desc0 + ((st * S::kTile) >> 4);
-            const bool last = pv.last() || in_flush + 1 == kFlush;
             if (leader) {
                 // Per page, P_hi then P_lo (chunks of 32 tokens: 16 columns
                 // of hi pairs, 16 of lo pairs).
@@ -363,18 +378,7 @@ prefix_tc_kernel(const __grid_constant__ PrefixParams p, const __grid_constant__
             }
             in_flush = last ? 0 : in_flush + 1;
             flush += last ? 1 : 0;
-            pv.step();
-            return true;
-        };
-        // QK runs two tiles ahead. PV(t) is committed before QK(t + 2) may
-        // wait for its segment's Q, which the staging warps write after
-        // reading the O that PV(t) may end.
-        bool ok = true;
-        for (uint32_t i = 0; ok && pv.valid(); ++i) {
-            if (i >= 2 || !qk.valid()) ok = pv_step();
-            if (ok && qk.valid()) ok = qk_step();
         }
-        // Every MMA this thread issued is complete before TMEM is released.
         if (leader) tc::commit(&mma_done);
         (void)wait(&mma_done, 0);
     } else if (warp >= 4 && warp < 8) {
@@ -614,15 +618,21 @@ prefix_tc_kernel(const __grid_constant__ PrefixParams p, const __grid_constant__
                     // sum = sum 2^(m_o - m) + O; a segment's first flush sets it.
                     const float alpha = m_o == ml.x ? 1.f : ex2_approx(m_o - ml.x);
                     const bool first = j == j0;
-#pragma unroll 1
+float v[HD];
+#pragma unroll
+                    for (uint32_t cb = 0; cb < HD; cb += 32) tc::ld32(tO + cb, v + cb);
+                    tc::wait_ld32(v);
+#pragma unroll
+                    for (uint32_t cb = 32; cb < HD; cb += 32) tc::reg_fence32(v + cb);
+                    // O is in registers: the next flush's PV may start.
+                    tc::fence_before_sync();
+                    mbar_arrive(&o_free);
+#pragma unroll
                     for (uint32_t cb = 0; cb < HD; cb += 32) {
-                        float v[32];
-                        tc::ld32(tO + cb, v);
-                        tc::wait_ld32(v);
                         float4* at = sum + cb * (kBM / 4) + lane * 8;
 #pragma unroll
                         for (uint32_t e = 0; e < 8; ++e) {
-                            float4 x = make_float4(v[4 * e], v[4 * e + 1], v[4 * e + 2], v[4 * e + 3]);
+                            float4 x = make_float4(v[cb + 4 * e], v[cb + 4 * e + 1], v[cb + 4 * e + 2], v[cb + 4 * e + 3]);
                             if (!first) {
                                 const float4 y = at[e ^ (lane & 7u)];
                                 x = make_float4(fmaf(y.x, alpha, x.x), fmaf(y.y, alpha, x.y), fmaf(y.z, alpha, x.z),
@@ -633,9 +643,10 @@ prefix_tc_kernel(const __grid_constant__ PrefixParams p, const __grid_constant__
                     }
                     m_o = ml.x;
                     l = ml.y;
+                } else {
+                    tc::fence_before_sync();
+                    mbar_arrive(&o_free);
                 }
-                tc::fence_before_sync();
-                mbar_arrive(&o_free);
             }
             if (ok && live) {
                 __syncwarp();
