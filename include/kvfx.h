@@ -259,9 +259,10 @@ int kvfx_decode(const kvfx_cache* cache, const float* q, float* o,
  *               bytes, 16-byte aligned; nothing is kept in it from call to
  *               call. Calls that share one must not overlap on the GPU.
  * The other arguments as for kvfx_decode. 16-bit caches with head_size 64 or
- * 128, block_size 16 and 16-byte aligned q and o read the prefix on the tensor cores (at
- * the FP32-class accuracy of the other attention entry points); other shapes
- * run row by row, each reading its whole table row. No counterpart in the
+ * 128 and block_size 16, with 16-byte aligned bases, q and o, read the prefix on
+ * the tensor cores (at the FP32-class accuracy of the other attention entry
+ * points), unless the rows are so short that reading them one by one is
+ * faster; other shapes run row by row, each reading its whole table row. No counterpart in the
  * reference, whose batch attention re-reads shared pages for every row
  * (src/v2/paged_attention.cu:248-313).
  */

@@ -37,7 +37,8 @@
 // Tail mode (kvfx_decode_shared): the same kernel over the pages behind each
 // row's shared prefix. A row's pages start at its group's prefix, every split
 // leaves its (max, sum, O) in the workspace, and the merge kernel of
-// shared.cu joins them with the prefix's. Query groups above 8 heads take one
+// shared.cu joins them with the prefix's; where no row has more than one
+// split, the CTA joins its piece with the prefix's itself. Query groups above 8 heads take one
 // CTA per 8 heads (blockIdx.y = KV head * chunks + chunk).
 #include <algorithm>
 #include <atomic>
@@ -107,7 +108,9 @@ struct PrefixTail {
     uint32_t q_group;     // query heads per KV head
     uint32_t chunks;      // CTAs per KV head: ceil(q_group / 8)
     uint32_t after_prefix;  // launched as a dependent of the prefix kernel
+    uint32_t fused;         // one split a row, joined with the prefix's pieces here
     uint32_t direct;        // no prefix kernel and one split a row: its pages from the first on, O written here
+    PrefixPieces pieces;
 };
 
 template <int HD, typename T, typename Tail>
@@ -172,15 +175,23 @@ decode_mma_kernel(const __grid_constant__ DecodeParams p, const __grid_constant_
             row0 = p.table + static_cast<uint64_t>(g == 0 ? 0 : tail.groups.row_end[g - 1]) * p.max_blocks;
         } else {
             first = pages;
-            // Rows outside the bounds are refused (and flagged) by the merge kernel.
-            if (len > tail.max_len || npages <= first) {
+            const bool outside = len > tail.max_len || npages > p.max_blocks || len < pages * 16;
+            if (tail.fused != 0) {
+                if (len == 0 || outside) {
+                    if (len != 0 && tid == 0) raise_flag(p.status, KVFX_FLAG_BAD_INDEX);
+                    pdl_wait();
+                    return;
+                }
+            } else if (outside || npages <= first) {  // refused (and flagged) by the merge kernel, or nothing to do
                 pdl_wait();
                 return;
             }
         }
     }
     const uint32_t nsplits = static_cast<uint32_t>(ceil_div(npages - first, p.pages_per_split));
-    if (len == 0 || split >= nsplits) {
+    bool none = len == 0 || split >= nsplits;
+    if constexpr (kTail) none = none && tail.fused == 0;  // a row without pages of its own still has its prefix
+    if (none) {
         if constexpr (kTail) pdl_wait();
         return;
     }
@@ -245,7 +256,7 @@ decode_mma_kernel(const __grid_constant__ DecodeParams p, const __grid_constant_
     // for a table read.
     const bool ids_cached = n_my <= 64;
     uint64_t id_lo = 0, id_hi = 0;
-    if (ids_cached) {
+    if (ids_cached || kTail) {
         const uint64_t j0 = pbeg + warp + static_cast<uint64_t>(kWarps) * lane;
         const uint64_t j1 = j0 + static_cast<uint64_t>(kWarps) * 32;
         if (lane < n_my) id_lo = append ? __ldcg(row + j0) : __ldg((kTail && j0 < shared ? row0 : row) + j0);
@@ -257,10 +268,16 @@ decode_mma_kernel(const __grid_constant__ DecodeParams p, const __grid_constant_
         if (i >= n_my) return;
         const uint64_t j = pbeg + warp + static_cast<uint64_t>(kWarps) * i;
         uint64_t blk;
-        if (ids_cached) {
-            blk = __shfl_sync(0xffffffffu, i < 32 ? id_lo : id_hi, i & 31);
+        if constexpr (kTail) {
+            if ((i & 31u) == 0 && i >= 64) {  // long splits: the next 32 ids
+                const uint64_t jl = j + static_cast<uint64_t>(kWarps) * lane;
+                if (i + lane < n_my) id_lo = __ldg((jl < shared ? row0 : row) + jl);
+            }
+        }
+        if (ids_cached || kTail) {
+            blk = __shfl_sync(0xffffffffu, i >= 32 && i < 64 ? id_hi : id_lo, i & 31);
         } else if (lane == 0) {
-            blk = append ? __ldcg(row + j) : __ldg((kTail && j < shared ? row0 : row) + j);
+            blk = append ? __ldcg(row + j) : __ldg(row + j);
         } else {
             blk = 0;
         }
@@ -466,6 +483,77 @@ decode_mma_kernel(const __grid_constant__ DecodeParams p, const __grid_constant_
     }
     __syncthreads();
 
+    if constexpr (kTail) {
+        if (tail.fused != 0) {
+            // This CTA's piece (its warps' O in mo, s_m[0], s_l[0]) and the
+            // prefix's segments, each weighted by 2^(m - M), over their sum.
+            pdl_wait();  // the prefix kernel has ended
+            if (failed) return;
+            const uint32_t g = tail.groups.of_row(static_cast<uint32_t>(r)), gq0 = qh0 - kh * tail.q_group;
+            float* weight = mo + kWarps * 8 * HD;  // [8][kMaxSplits], the last one this CTA's own
+            for (uint32_t gg = warp; gg < G; gg += kWarps) {
+                uint64_t row;
+                uint32_t n;
+                tail.pieces.of_row(tail.groups, g, static_cast<uint32_t>(r), kh, gq0 + gg, tail.q_group, &row, &n);
+                const float2* ml = reinterpret_cast<const float2*>(tail.pieces.part_ml) + row;
+                float M = s_m[0][gg];
+                for (uint32_t i = lane; i < n; i += 32) M = fmaxf(M, __ldcg(ml + i * 128).x);
+#pragma unroll
+                for (int x = 16; x > 0; x >>= 1) M = fmaxf(M, __shfl_xor_sync(0xffffffffu, M, x));
+                float L = 0.f;
+                for (uint32_t i = lane; i < n; i += 32) {
+                    const float2 piece = __ldcg(ml + i * 128);
+                    const float w = piece.x == -INFINITY ? 0.f : exp2f(piece.x - M);
+                    weight[gg * kMaxSplits + i] = w;
+                    if (w != 0.f) L = fmaf(piece.y, w, L);
+                }
+#pragma unroll
+                for (int x = 16; x > 0; x >>= 1) L += __shfl_xor_sync(0xffffffffu, L, x);
+                const float w = s_m[0][gg] == -INFINITY ? 0.f : exp2f(s_m[0][gg] - M);
+                if (w != 0.f) L = fmaf(s_l[0][gg], w, L);
+                const float inv = 1.f / L;
+                // Two dims a lane (of HD / 64 pairs), four pieces' loads ahead.
+                const float2* po = reinterpret_cast<const float2*>(tail.pieces.part_o + row * HD) + lane;
+                float2 acc[HD / 64];
+                __syncwarp();
+#pragma unroll
+                for (int v = 0; v < HD / 64; ++v) {
+                    acc[v] = make_float2(0.f, 0.f);
+                    if (w == 0.f) continue;
+#pragma unroll
+                    for (int ww = 0; ww < kWarps; ++ww) {
+                        const float2 x = reinterpret_cast<const float2*>(mo + (ww * 8 + gg) * HD)[lane + 32 * v];
+                        acc[v].x = fmaf(x.x, s_scale[ww][gg] * w, acc[v].x);
+                        acc[v].y = fmaf(x.y, s_scale[ww][gg] * w, acc[v].y);
+                    }
+                }
+                for (uint32_t i = 0; i < n; i += 4) {
+                    float2 x[4][HD / 64];
+#pragma unroll
+                    for (int a = 0; a < 4; ++a) {
+#pragma unroll
+                        for (int v = 0; v < HD / 64; ++v)
+                            if (i + a < n) x[a][v] = __ldcg(po + static_cast<uint64_t>(i + a) * 64 * HD + 32 * v);
+                    }
+#pragma unroll
+                    for (int a = 0; a < 4; ++a) {
+                        const float wa = i + a < n ? weight[gg * kMaxSplits + i + a] : 0.f;
+                        if (wa == 0.f) continue;  // whatever such a piece holds
+#pragma unroll
+                        for (int v = 0; v < HD / 64; ++v) {
+                            acc[v].x = fmaf(x[a][v].x, wa, acc[v].x);
+                            acc[v].y = fmaf(x[a][v].y, wa, acc[v].y);
+                        }
+                    }
+                }
+                float2* out = reinterpret_cast<float2*>(
+                    p.o + (r * p.kv_heads * tail.q_group + qh0 + gg) * HD);
+#pragma unroll
+                for (int v = 0; v < HD / 64; ++v) out[lane + 32 * v] = make_float2(acc[v].x * inv, acc[v].y * inv);
+            }
+            return;
+        }
+    }
     const uint64_t pair = r * (kTail ? gridDim.y : p.kv_heads) + (kTail ? blockIdx.y : kh);
     if (alone) {
         for (uint32_t idx = tid; idx < G * HD; idx += kWarps * 32) {
@@ -649,7 +737,8 @@ cudaError_t launch_tail(const CacheView& c, const TailArgs& a, const CacheMaps* 
     p.partial = a.partial;
     p.status = status;
     const uint32_t q_group = a.q_heads / c.heads, chunks = (q_group + 7) / 8;
-    const PrefixTail tail{*a.groups, a.max_len, q_group, chunks, a.after_prefix ? 1u : 0u, a.direct ? 1u : 0u};
+    const PrefixTail tail{*a.groups, a.max_len, q_group, chunks, a.after_prefix ? 1u : 0u, a.fused ? 1u : 0u,
+                          a.direct ? 1u : 0u, a.pieces};
     cudaLaunchConfig_t cfg{};
     cfg.gridDim = dim3(a.max_splits, c.heads * chunks, a.groups->rows());
     cfg.blockDim = dim3(kWarps * 32);

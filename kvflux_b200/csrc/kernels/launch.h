@@ -154,10 +154,43 @@ struct PrefixGroups {
     __host__ __device__ uint32_t of_tile(uint32_t tile) const { return find(tile_end, tile); }
 };
 
+// The segments a query row's prefix was attended in: n of them, 128 rows of
+// part_o and part_ml apart from row `first` on.
+struct PrefixPieces {
+    const float* part_o;
+    const float* part_ml;
+    uint64_t tiles_inv;  // floor(2^64 / tiles)
+    uint32_t grid;       // CTAs of the prefix launch (0: nothing shared)
+
+    __device__ __forceinline__ void of_row(const PrefixGroups& gs, uint32_t g, uint32_t row, uint32_t kh, uint32_t gq,
+                                           uint32_t q_group, uint64_t* first, uint32_t* n) const {
+        *first = 0;
+        *n = 0;
+        if (gs.pages[g] == 0) return;
+        const uint32_t row0 = g == 0 ? 0 : gs.row_end[g - 1];
+        const uint32_t tile0 = g == 0 ? 0 : gs.tile_end[g - 1], pair0 = g == 0 ? 0 : gs.pair_end[g - 1];
+        const uint32_t m = (row - row0) * q_group + gq;  // query row in the group's matrix
+        const uint32_t pair = kh * (((gs.row_end[g] - row0) * q_group + 127) / 128) + m / 128;
+        const uint32_t ntiles = (gs.pages[g] + 7) / 8;
+        // The CTAs whose runs [tiles c / grid, tiles (c + 1) / grid) meet the pair's tiles.
+        const uint32_t tiles = gs.tiles(), t0 = tile0 + pair * ntiles;
+        auto owner = [&](uint32_t t) {
+            const uint64_t x = (static_cast<uint64_t>(t) + 1) * grid - 1;
+            uint64_t c = __umul64hi(x, tiles_inv);  // x / tiles, or one less
+            if (x - c * tiles >= tiles) ++c;
+            return static_cast<uint32_t>(c);
+        };
+        const uint32_t c0 = owner(t0);
+        *n = owner(t0 + ntiles - 1) - c0 + 1;
+        *first = static_cast<uint64_t>(c0 + pair0 + pair) * 128 + m % 128;
+    }
+};
+
 // The rows' own pages behind their groups' prefixes (decode.cu, tail mode):
 // split s of (row, KV head and chunk y) leaves its partial, 8 (hd + 2)
-// floats, at partial[((row * gridDim.y + y) * max_splits + s)]. `direct`: all
-// of a row's pages instead, in one split whose O goes to o.
+// floats, at partial[((row * gridDim.y + y) * max_splits + s)]. `fused` (one
+// split a row): the split is joined with the prefix's pieces at once, and O
+// goes to o. `direct`: all of a row's pages, in one split whose O goes to o.
 struct TailArgs {
     const float* q;
     float* o;
@@ -167,7 +200,8 @@ struct TailArgs {
     uint32_t q_heads, pages_per_split, max_splits;
     const PrefixGroups* groups;
     float* partial;
-    bool after_prefix, direct;
+    PrefixPieces pieces;
+    bool after_prefix, fused, direct;
 };
 // A split size the kernel takes, near `pps`, for rows of at most max_pages.
 uint32_t decode_tail_split(const CacheView& c, uint64_t max_pages, uint32_t pps);

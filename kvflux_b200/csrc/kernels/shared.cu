@@ -7,7 +7,9 @@
 // Three launches, each a programmatic dependent of the one before it:
 //   prefix  (prefix.cu)   the groups' shared pages, once per 128 query rows;
 //   tail    (decode.cu)   each row's own pages behind them;
-//   merge   (below)       the pieces of every (row, query head).
+//   merge   (below)       the pieces of every (row, query head), where a row
+//                         may have several of its own (else the tail's CTAs
+//                         join theirs with the prefix's).
 // The workspace holds the pieces only, so nothing in it outlives a call.
 #include <algorithm>
 #include <cmath>
@@ -19,18 +21,16 @@ namespace kvfx {
 namespace {
 
 constexpr int kMergeWarps = 4;
+constexpr uint32_t kFirstCtas = 1024;  // about one wave
 constexpr uint32_t kAhead = 8;  // pieces' O in flight
 
 struct MergeParams {
     PrefixGroups groups;
     const uint64_t* lens;
     float* o;
-    const float* part_o;   // prefix segments: [slot][128][hd], [slot][128][2]
-    const float* part_ml;
+    PrefixPieces pieces;   // prefix segments
     const float* tail;     // tail splits: [row][heads x chunks][split][8][hd + 2]
     uint64_t max_len, max_blocks;
-    uint64_t tiles_inv;    // floor(2^64 / tiles)
-    uint32_t grid;         // CTAs of the prefix launch
     uint32_t q_heads, kv_heads, q_group, chunks;
     uint32_t pages_per_split, max_splits;
     unsigned* status;
@@ -62,27 +62,9 @@ __global__ void __launch_bounds__(kMergeWarps * 32) merge_kernel(const __grid_co
     }
     // The row's pieces in order: its prefix segments, then its own splits.
     const uint32_t kh = j / p.q_group, gq = j - kh * p.q_group;
-    uint32_t n_seg = 0;
-    uint64_t seg_row = 0;  // first segment's row of part_o
-    if (first != 0) {
-        const uint32_t row0 = g == 0 ? 0 : p.groups.row_end[g - 1];
-        const uint32_t tile0 = g == 0 ? 0 : p.groups.tile_end[g - 1], pair0 = g == 0 ? 0 : p.groups.pair_end[g - 1];
-        const uint32_t rows = (p.groups.row_end[g] - row0) * p.q_group;
-        const uint32_t m = (row - row0) * p.q_group + gq;  // query row in the group's matrix
-        const uint32_t pair = kh * ((rows + 127) / 128) + m / 128;
-        const uint32_t ntiles = (first + 7) / 8;
-        // The CTAs whose runs [tiles c / grid, tiles (c + 1) / grid) meet the pair's tiles.
-        const uint32_t tiles = p.groups.tiles(), t0 = tile0 + pair * ntiles;
-        auto owner = [&](uint32_t t) {
-            const uint64_t x = (static_cast<uint64_t>(t) + 1) * p.grid - 1;
-            uint64_t c = __umul64hi(x, p.tiles_inv);  // x / tiles, or one less
-            if (x - c * tiles >= tiles) ++c;
-            return static_cast<uint32_t>(c);
-        };
-        const uint32_t c0 = owner(t0);
-        n_seg = owner(t0 + ntiles - 1) - c0 + 1;
-        seg_row = static_cast<uint64_t>(c0 + pair0 + pair) * 128 + m % 128;
-    }
+    uint32_t n_seg;
+    uint64_t seg_row;  // first segment's row of part_o
+    p.pieces.of_row(p.groups, g, row, kh, gq, p.q_group, &seg_row, &n_seg);
     const uint32_t own_pages = static_cast<uint32_t>(npages) - first;
     const uint32_t n = n_seg + (own_pages + p.pages_per_split - 1) / p.pages_per_split;
     const uint64_t unit = static_cast<uint64_t>(row) * (p.kv_heads * p.chunks) + kh * p.chunks + gq / 8;
@@ -98,16 +80,21 @@ __global__ void __launch_bounds__(kMergeWarps * 32) merge_kernel(const __grid_co
     // it brings the loop's code and the kernel's parameters into the caches
     // while the launches ahead run (they stream more K and V than the L2
     // holds, so what is missing here would come from HBM, line after line).
+    // (Only the first CTAs: the later ones find everything there.)
     uint32_t warm, base = 0;
     asm volatile("mov.u32 %0, 0;" : "=r"(warm) : "r"(n));  // unknown to the compiler: one copy of the loop; n is there
+    if (blockIdx.x >= kFirstCtas) {
+        warm = 1;
+        pdl_wait();
+    }
 #pragma unroll 1
     do {
         const uint32_t here = warm != 0 ? min(32u, n - base) : 1u;
         const uint32_t i = base + lane;
         const uint64_t r = seg_row + static_cast<uint64_t>(i) * 128;
         const float* split = tail + static_cast<int64_t>(static_cast<int32_t>(i - n_seg)) * 8 * (HD + 2);
-        const float* o = i < n_seg ? p.part_o + r * HD : split;
-        const float* at = i < n_seg ? p.part_ml + r * 2 : split + HD;
+        const float* o = i < n_seg ? p.pieces.part_o + r * HD : split;
+        const float* at = i < n_seg ? p.pieces.part_ml + r * 2 : split + HD;
         if (warm == 0) o = at = reinterpret_cast<const float*>(out);
         float2 ml = make_float2(-INFINITY, 0.f);
         if (lane < here) ml = __ldcg(reinterpret_cast<const float2*>(at));
@@ -174,6 +161,7 @@ struct Plan {
     PrefixGroups groups;
     bool direct;               // one launch, each row reading all of its pages
     uint32_t grid;             // prefix CTAs (0: nothing shared)
+    bool fused;                // the tail's CTAs write O
     bool stream;               // no group has more than one tile of query rows
     uint32_t pages_per_split;  // tail splits
     uint32_t max_splits;       // 0: no row has pages of its own
@@ -193,11 +181,12 @@ bool make_plan(const CacheView& c, const kvfx_prefix_group* groups, uint32_t n, 
     PrefixGroups& gs = plan->groups;
     plan->stream = true;
     gs.n = n;
-    uint64_t rows = 0, pairs = 0, tiles = 0, tail_pages = 0;
+    uint64_t rows = 0, pairs = 0, tiles = 0, tail_pages = 0, longest = 0;
     for (uint32_t g = 0; g < n; ++g) {
         const uint64_t pages = groups[g].prefix_tokens / 16;
         const uint64_t group_pairs = pages != 0 ? c.heads * ceil_div(groups[g].rows * q_group, 128) : 0;
         rows += groups[g].rows;
+        longest = std::max(longest, pages);
         pairs += group_pairs;
         if (group_pairs > c.heads) plan->stream = false;
         tiles += group_pairs * ceil_div(pages, 8);
@@ -217,6 +206,7 @@ bool make_plan(const CacheView& c, const kvfx_prefix_group* groups, uint32_t n, 
     plan->direct = max_pages <= 40 && rows * c.heads * ceil_div(q_group, 8) <=
                                           3 * static_cast<uint64_t>(device_sm_count(c.device));
     if (plan->direct) {
+        plan->fused = false;
         plan->grid = 0;
         plan->pages_per_split = decode_tail_split(c, max_pages, static_cast<uint32_t>(max_pages));
         plan->max_splits = 1;
@@ -229,16 +219,28 @@ bool make_plan(const CacheView& c, const kvfx_prefix_group* groups, uint32_t n, 
     plan->pages_per_split = 1;
     plan->max_splits = 0;
     if (tail_pages != 0) {
-        plan->pages_per_split = decode_tail_split(
-            c, tail_pages, decode_pages_per_split(c, rows, q_heads, tail_pages * 16, 0));
+        // One split a row, whose CTA joins the prefix's pieces itself (no
+        // merge kernel), where it is short or the rows fill the GPU anyway:
+        // 256 rows x 64 heads behind 16384 tokens 385 us against 410 with the
+        // merge kernel, 64 rows x 32 heads behind 8 prompts 62 / 64. Few rows
+        // of some length are better split (16 rows x 8 KV heads of up to 32
+        // pages: 18.5 fused, 16.5 split).
+        const uint64_t ctas = rows * c.heads * ceil_div(q_group, 8);
+        uint32_t pps = decode_pages_per_split(c, rows, q_heads, tail_pages * 16, 0);
+        if (tail_pages <= 16 || (tail_pages <= 512 && ctas >= 2 * static_cast<uint64_t>(device_sm_count(c.device)))) {
+            pps = static_cast<uint32_t>(tail_pages);
+        }
+        plan->pages_per_split = decode_tail_split(c, tail_pages, pps);
         plan->max_splits = static_cast<uint32_t>(ceil_div(tail_pages, plan->pages_per_split));
     }
+    // (A fused CTA keeps at most 256 segments' weights: 148 CTAs' runs, or runs of 256 tiles.)
+    plan->fused = plan->max_splits == 1 && longest <= 1u << 19;
     const uint64_t slots = plan->grid != 0 ? plan->grid + pairs : 0;
     auto align = [](uint64_t b) { return (b + 255) & ~uint64_t(255); };
     plan->off_ml = align(slots * 128 * c.hd * 4);
     plan->off_tail = plan->off_ml + align(slots * 128 * 8);
     plan->bytes = plan->off_tail +
-                  align(rows * c.heads * ceil_div(q_group, 8) * plan->max_splits * 8 * (c.hd + 2) * 4);
+                  (plan->fused ? 0 : align(rows * c.heads * ceil_div(q_group, 8) * plan->max_splits * 8 * (c.hd + 2) * 4));
     return true;
 }
 
@@ -259,7 +261,8 @@ uint64_t shared_workspace_bytes(const CacheView& c, const kvfx_prefix_group* gro
 
 cudaError_t launch_decode_shared(const CacheView& c, const SharedArgs& a, unsigned* status, cudaStream_t s) {
     Plan plan;
-    const bool aligned = ((reinterpret_cast<uintptr_t>(a.q) | reinterpret_cast<uintptr_t>(a.o)) & 15u) == 0;
+    const bool aligned = ((reinterpret_cast<uintptr_t>(a.q) | reinterpret_cast<uintptr_t>(a.o) |
+                           reinterpret_cast<uintptr_t>(c.k) | reinterpret_cast<uintptr_t>(c.v)) & 15u) == 0;
     if (!make_plan(c, a.groups, a.num_groups, a.q_heads, a.max_len, &plan) || !aligned) {
         // Row by row over the whole table.
         uint64_t rows = 0;
@@ -282,24 +285,23 @@ cudaError_t launch_decode_shared(const CacheView& c, const SharedArgs& a, unsign
         err = launch_prefix_tc(c, pa, *groups, status, s);
         if (err != cudaSuccess) return err;
     }
+    const uint32_t tiles = plan.groups.tiles();
+    const uint64_t tiles_inv = tiles > 1 ? ~0ull / tiles + (~0ull % tiles == tiles - 1 ? 1 : 0) : ~0ull;
+    const PrefixPieces pieces{part_o, part_ml, tiles_inv, plan.grid};
     if (plan.max_splits != 0) {
         const TailArgs ta{a.q, a.o, a.table, a.lens, a.max_blocks, a.max_len, a.q_heads, plan.pages_per_split,
-                          plan.max_splits, &plan.groups, tail, plan.grid != 0, plan.direct};
+                          plan.max_splits, &plan.groups, tail, pieces, plan.grid != 0, plan.fused, plan.direct};
         err = launch_decode_tail(c, ta, *maps, status, s);
-        if (err != cudaSuccess || plan.direct) return err;
+        if (err != cudaSuccess || plan.direct || plan.fused) return err;
     }
     MergeParams m;
     m.groups = plan.groups;
     m.lens = a.lens;
     m.o = a.o;
-    m.part_o = part_o;
-    m.part_ml = part_ml;
+    m.pieces = pieces;
     m.tail = tail;
     m.max_len = a.max_len;
     m.max_blocks = a.max_blocks;
-    m.grid = plan.grid;
-    const uint32_t tiles = plan.groups.tiles();
-    m.tiles_inv = tiles > 1 ? ~0ull / tiles + (~0ull % tiles == tiles - 1 ? 1 : 0) : ~0ull;
     m.q_heads = a.q_heads;
     m.kv_heads = c.heads;
     m.q_group = a.q_heads / c.heads;

@@ -143,6 +143,22 @@ def test_against_every_row_alone(groups, lens, heads, group, hd, bs, dtype, room
     assert torch.equal(got, b.run())  # the same bits again
 
 
+@pytest.mark.parametrize("groups,lens,heads,group,hd", [
+    # rows that fill the GPU: one split a row, joined by its own CTA; some with nothing of their own, some refused later
+    ([(100, 320), (60, 0), (40, 16)], [320 + 5 * i % 700 if i < 100 else 16 + 11 * i % 900 for i in range(200)], 2, 3, 64),
+    # short rows of few: likewise
+    ([(5, 800)], [800, 801, 1000, 1056, 816], 1, 8, 128),
+    # few rows, long of their own: several splits and the merge kernel
+    ([(3, 160)], [6000, 160, 3000], 2, 9, 64),
+    # one row's split longer than 64 pages a warp
+    ([(300, 32)], [32 + (i % 3) for i in range(299)] + [5200], 1, 1, 64),
+])
+def test_one_split_a_row_and_several(groups, lens, heads, group, hd):
+    b = Batch(groups, lens, heads, group, hd)
+    b.check(b.run())
+    assert kv.device_status(0) == 0
+
+
 @pytest.mark.parametrize("dtype,hd", [("bfloat16", 128), ("float16", 64)])
 def test_large_and_growing_scores(dtype, hd):
     groups, lens = [(5, 1200)], [1200, 1201, 1300, 1250, 1216]
