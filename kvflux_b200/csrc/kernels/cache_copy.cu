@@ -9,7 +9,12 @@
 // never look at the element type. One launch covers every layer: blockIdx.y
 // is the layer, whose bases come from the kernel parameters, and blockIdx.z
 // the cache (K or V), which doubles the CTAs of a small copy. Work is a flat
-// range of vectors, so that pages of any size fill their CTAs.
+// range of vectors, so that pages of any size fill their CTAs, two vectors a
+// thread: small CTAs end evenly. B200, in a graph: 8190 tokens in 16 layers
+// 164 us, 6.56 TB/s read and written (1.00 of the plain copy rate; 165 / 173 us
+// with 4 / 8 vectors), 96 pages from 24 in 32 layers 42.8 us (201 MB written,
+// the repeated sources read from the L2; 42.4 / 43.3), 8 pages in one layer
+// 1.8 us (2.2 / 2.9).
 #include <algorithm>
 
 #include "common.cuh"
@@ -19,7 +24,7 @@ namespace kvfx {
 namespace {
 
 constexpr int kThreads = 256;
-constexpr int kPer = 4;  // vectors in flight per thread before its first store
+constexpr int kPer = 2;  // vectors in flight per thread before its first store
 
 template <int VB>
 __global__ void __launch_bounds__(kThreads) copy_pages_kernel(const __grid_constant__ LayerBases bases,
