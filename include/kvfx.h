@@ -193,13 +193,14 @@ int kvfx_rotary_table(float* cos_sin, uint64_t max_positions, uint32_t rotary_di
  *               cache or q_out
  *   positions : device uint64[num_tokens], each < max_positions
  *   slots     : device uint64[num_tokens], pairwise distinct; KVFX_NO_SLOT
- *               marks a padding token: nothing of it is read or written
+ *               marks a padding token: nothing is written for it, and
+ *               its position, q, k and v may hold anything
  *   q_out     : device float[num_tokens][q_heads][head_size]
  * q_heads may be 0 (q and q_out are then not looked at). A token whose slot
  * or position is out of range is skipped and sets KVFX_FLAG_BAD_INDEX.
  * Rows of 32, 64, 128 or 256 elements with 16-byte aligned bases and strides
- * (q_out: 32-byte), and a rotary_dim that is a multiple of 16 (8 interleaved), take a kernel of
- * 16-byte vectors; other shapes an element-wise one.
+ * (q_out: 32-byte), and a rotary_dim that is a multiple of 16 (8 interleaved),
+ * take a kernel of 16-byte vectors; other shapes an element-wise one.
  * No counterpart in the reference, whose write takes K and V as they are
  * (src/v2/paged_kv_write.cu:101-139).
  */
@@ -246,7 +247,8 @@ int kvfx_decode(const kvfx_cache* cache, const float* q, float* o,
  * instead of once per row. Group g is the next groups[g].rows rows of the
  * batch, whose first groups[g].prefix_tokens positions (whole pages) are the
  * same pages: those of the group's first row, whose table entries are read
- * for them; every row's table still holds all of its pages. The batch is the
+ * for them (also where that row is padding); every row's table still holds all
+ * of its pages. The batch is the
  * groups' rows in order (at most 65535), num_groups at most
  * KVFX_MAX_PREFIX_GROUPS, prefix_tokens a multiple of block_size, at most
  * max_seq_len, and 0 where rows share nothing. groups is a host array, read
@@ -262,9 +264,9 @@ int kvfx_decode(const kvfx_cache* cache, const float* q, float* o,
  * 128 and block_size 16, with 16-byte aligned bases, q and o, read the prefix on
  * the tensor cores (at the FP32-class accuracy of the other attention entry
  * points), unless the rows are so short that reading them one by one is
- * faster; other shapes run row by row, each reading its whole table row. No counterpart in the
- * reference, whose batch attention re-reads shared pages for every row
- * (src/v2/paged_attention.cu:248-313).
+ * faster; other shapes run row by row, each reading its whole table row.
+ * No counterpart in the reference, whose batch attention re-reads shared pages
+ * for every row (src/v2/paged_attention.cu:248-313).
  */
 typedef struct kvfx_prefix_group {
     uint64_t rows;           /* >= 1 */

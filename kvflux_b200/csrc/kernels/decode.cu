@@ -38,8 +38,8 @@
 // row's shared prefix. A row's pages start at its group's prefix, every split
 // leaves its (max, sum, O) in the workspace, and the merge kernel of
 // shared.cu joins them with the prefix's; where no row has more than one
-// split, the CTA joins its piece with the prefix's itself. Query groups above 8 heads take one
-// CTA per 8 heads (blockIdx.y = KV head * chunks + chunk).
+// split, the CTA joins its piece with the prefix's itself. Query groups above
+// 8 heads take one CTA per 8 heads (blockIdx.y = KV head * chunks + chunk).
 #include <algorithm>
 #include <atomic>
 #include <cmath>
@@ -397,7 +397,8 @@ decode_mma_kernel(const __grid_constant__ DecodeParams p, const __grid_constant_
         const bool need = mx > m_run + 8.f;
         if (__any_sync(0xffffffffu, need)) {
             const float m_new = need ? mx : m_run;
-            const float alpha = exp2f(m_run - m_new);
+            float alpha = exp2f(m_run - m_new);
+            if constexpr (kTail) alpha = need ? alpha : 1.f;  // (both may be -inf)
             l_run *= alpha;
 #pragma unroll
             for (int n = 0; n < S::kNTiles; ++n) {
@@ -409,10 +410,12 @@ decode_mma_kernel(const __grid_constant__ DecodeParams p, const __grid_constant_
             m_run = m_new;
         }
         float pw[2][2];
+        float m_sub = m_run;
+        if constexpr (kTail) m_sub = m_run == -INFINITY ? 0.f : m_run;  // scores of -inf so far: weights of 0
 #pragma unroll
         for (int nt = 0; nt < 2; ++nt) {
-            pw[nt][0] = exp2f(s[nt][0] - m_run);
-            pw[nt][1] = exp2f(s[nt][1] - m_run);
+            pw[nt][0] = exp2f(s[nt][0] - m_sub);
+            pw[nt][1] = exp2f(s[nt][1] - m_sub);
             l_run += pw[nt][0] + pw[nt][1];
         }
         uint32_t pa[4];
@@ -505,12 +508,12 @@ decode_mma_kernel(const __grid_constant__ DecodeParams p, const __grid_constant_
                     const float2 piece = __ldcg(ml + i * 128);
                     const float w = piece.x == -INFINITY ? 0.f : exp2f(piece.x - M);
                     weight[gg * kMaxSplits + i] = w;
-                    if (w != 0.f) L = fmaf(piece.y, w, L);
+                    L = fmaf(piece.y, w, L);  // (NaN, from scores of NaN, comes through)
                 }
 #pragma unroll
                 for (int x = 16; x > 0; x >>= 1) L += __shfl_xor_sync(0xffffffffu, L, x);
                 const float w = s_m[0][gg] == -INFINITY ? 0.f : exp2f(s_m[0][gg] - M);
-                if (w != 0.f) L = fmaf(s_l[0][gg], w, L);
+                L = fmaf(s_l[0][gg], w, L);
                 const float inv = 1.f / L;
                 // Two dims a lane (of HD / 64 pairs), four pieces' loads ahead.
                 const float2* po = reinterpret_cast<const float2*>(tail.pieces.part_o + row * HD) + lane;

@@ -45,8 +45,9 @@
 // 256 rows x 64 heads.) A flush takes all of O into registers and lets the
 // next PV go before it adds: 208 us against 218 at 256 rows x 64 heads x 16384
 // tokens, 620 -> 660 TFLOP/s of attention (twice that executed), where a tile
-// is bounded by its chain: softmax 1.2 us, PV and QK 0.6 us each. O is rescaled in TMEM only when a tile's row maximum
-// passes the running one by more than 8.
+// is bounded by its chain: softmax 1.2 us, PV and QK 0.6 us each. O is
+// rescaled in TMEM only when a tile's row maximum passes the running one by
+// more than 8.
 #include <algorithm>
 #include <atomic>
 #include <cmath>
@@ -459,7 +460,7 @@ prefix_tc_kernel(const __grid_constant__ PrefixParams p, const __grid_constant__
                 // P over its own S columns: chunk of 32 tokens -> 16 columns
                 // of hi pairs, 16 of lo pairs. The scores are read again
                 // chunk by chunk, the next one's load under this one's math.
-                const float m_sub = m_run == -INFINITY ? 0.f : m_run;  // no visible score yet: weights of 0
+                const float m_sub = m_run == -INFINITY ? 0.f : m_run;  // no score above -inf yet: weights of 0
                 const uint64_t mm = f2_pack(m_sub, m_sub);
                 uint64_t sum0 = f2_pack(0.f, 0.f), sum1 = sum0;
                 auto p_chunk = [&](int ch, float* v) {
@@ -618,7 +619,7 @@ prefix_tc_kernel(const __grid_constant__ PrefixParams p, const __grid_constant__
                     // sum = sum 2^(m_o - m) + O; a segment's first flush sets it.
                     const float alpha = m_o == ml.x ? 1.f : ex2_approx(m_o - ml.x);
                     const bool first = j == j0;
-float v[HD];
+                    float v[HD];
 #pragma unroll
                     for (uint32_t cb = 0; cb < HD; cb += 32) tc::ld32(tO + cb, v + cb);
                     tc::wait_ld32(v);

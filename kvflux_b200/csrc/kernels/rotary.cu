@@ -147,6 +147,7 @@ __device__ __forceinline__ uint64_t slot_row(const RotatedParams& p, uint64_t sl
 //     y_d = (x_d a_d + x_partner(d) b_d) / sqrt(mean(x^2) + eps),
 // a = w c and b = +- w_partner s, and the partner's x comes as stored (16-bit
 // rows: four shuffles a row, and half the instructions of norming first).
+// Lanes past rotary_dim take 0 for it: an infinity there stays as it is.
 template <typename T, int LPR>
 __global__ void __launch_bounds__(kThreads, kMinCtas) write_rotated_kernel(const __grid_constant__ RotatedParams p) {
     constexpr int kGroups = kThreads / LPR;
@@ -188,6 +189,7 @@ __global__ void __launch_bounds__(kThreads, kMinCtas) write_rotated_kernel(const
     const int rot = static_cast<int>(p.rotary_dim), half = rot / 2;
     uint64_t qa[kEl / 2], qb[kEl / 2], ka[kEl / 2], kb[kEl / 2];
     int partner = l;
+    const uint32_t turned = d0 < rot ? ~0u : 0u;
     {
         const float* tab = p.cos_sin + pos * p.rotary_dim;
         uint64_t c[kEl / 2], s[kEl / 2];
@@ -262,13 +264,13 @@ __global__ void __launch_bounds__(kThreads, kMinCtas) write_rotated_kernel(const
             }
             if (p.interleaved) {
 #pragma unroll
-                for (int e = 0; e < kEl / 2; ++e) y[e] = f2_swap(x[e]);
+                for (int e = 0; e < kEl / 2; ++e) y[e] = turned != 0 ? f2_swap(x[e]) : 0;
             } else {
                 Raw<T> other;
                 uint32_t* to = reinterpret_cast<uint32_t*>(other.w);
                 const uint32_t* from = reinterpret_cast<const uint32_t*>(raw[i].w);
 #pragma unroll
-                for (int e = 0; e < static_cast<int>(sizeof(Raw<T>) / 4); ++e) to[e] = __shfl_sync(lanes, from[e], partner, LPR);
+                for (int e = 0; e < static_cast<int>(sizeof(Raw<T>) / 4); ++e) to[e] = __shfl_sync(lanes, from[e], partner, LPR) & turned;
                 widen8<T>(other, y);
             }
             const uint64_t scale2 = f2_pack(scale, scale);

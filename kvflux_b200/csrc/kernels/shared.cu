@@ -4,12 +4,14 @@
 // prefix, and each side further; a piece with running maximum m, sum l and
 // unnormalised O joins the others by
 //     M = max m,  L = sum l 2^(m - M),  o = (sum O 2^(m - M)) / L.
-// Three launches, each a programmatic dependent of the one before it:
+// One to three launches, each a programmatic dependent of the one before it:
 //   prefix  (prefix.cu)   the groups' shared pages, once per 128 query rows;
 //   tail    (decode.cu)   each row's own pages behind them;
-//   merge   (below)       the pieces of every (row, query head), where a row
-//                         may have several of its own (else the tail's CTAs
-//                         join theirs with the prefix's).
+//   merge   (below)       the pieces of every (row, query head).
+// Where no row has more than one split of its own, the tail's CTAs join it
+// with the prefix's pieces and write O ("fused"), and the merge is left out;
+// where the rows are short and few, the tail reads all of their pages, shared
+// ones too ("direct"), and is the only launch. make_plan has the rules.
 // The workspace holds the pieces only, so nothing in it outlives a call.
 #include <algorithm>
 #include <cmath>
@@ -104,10 +106,9 @@ __global__ void __launch_bounds__(kMergeWarps * 32) merge_kernel(const __grid_co
         m_new = fmaxf(m_new, M);
         const float keep = M == -INFINITY ? 0.f : exp2f(M - m_new);
         M = m_new;
-        // A piece without any visible score (m = -inf) weighs nothing,
-        // whatever its O holds.
+        // A piece whose scores are all -inf weighs nothing, whatever its O holds.
         const float w = ml.x == -INFINITY ? 0.f : exp2f(ml.x - M);
-        float sum = w != 0.f ? ml.y * w : 0.f;
+        float sum = ml.y * w;  // (l is 0 there, or NaN from scores of NaN, which must come through)
 #pragma unroll
         for (int s = 16; s > 0; s >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, s);
         L = fmaf(L, keep, sum);
@@ -233,8 +234,10 @@ bool make_plan(const CacheView& c, const kvfx_prefix_group* groups, uint32_t n, 
         plan->pages_per_split = decode_tail_split(c, tail_pages, pps);
         plan->max_splits = static_cast<uint32_t>(ceil_div(tail_pages, plan->pages_per_split));
     }
-    // (A fused CTA keeps at most 256 segments' weights: 148 CTAs' runs, or runs of 256 tiles.)
-    plan->fused = plan->max_splits == 1 && longest <= 1u << 19;
+    // A fused CTA keeps at most 256 segments' weights. A prefix of 2^18 pages
+    // has 2^15 tiles, which lie in at most 148 runs, or, where there are more
+    // CTAs, in runs of 254 to 256 tiles: at most 131 of them.
+    plan->fused = plan->max_splits == 1 && longest <= 1u << 18;
     const uint64_t slots = plan->grid != 0 ? plan->grid + pairs : 0;
     auto align = [](uint64_t b) { return (b + 255) & ~uint64_t(255); };
     plan->off_ml = align(slots * 128 * c.hd * 4);

@@ -158,6 +158,22 @@ def test_bad_slots_and_positions_are_skipped_and_flagged():
     assert same.all()
 
 
+def test_an_infinity_past_rotary_dim_stays():
+    for dtype, inter in (("float16", 0), ("bfloat16", 1), ("float32", 0)):
+        c = Cache(4, 1, 16, 128, dtype, seed=23)
+        q = torch.randn(3, 2 * 128).to(TORCH[dtype]).cuda()
+        k, v = q[:, :128].contiguous(), q[:, 128:].contiguous()
+        q[1, 100], k[2, 64], q[0, 127] = float("inf"), float("-inf"), float("inf")
+        tab = torch.tensor(table64(8, 64), dtype=torch.float32, device="cuda")
+        out = torch.zeros(3, 2, 128, device="cuda")
+        rotary = kv.KvfxRotary(tab.data_ptr(), 8, 64, inter, None, None, 0.0, 0)
+        call(kv.lib.kvfx_write_rotated, ctypes.byref(c.desc), ctypes.byref(rotary), q, k, v, 256, 128, 128, 2, u64(np.arange(3)), u64(np.arange(3)), 3, out, None)
+        assert torch.equal(out[:, :, 64:], q.view(3, 2, 128)[:, :, 64:].float())
+        assert torch.all(torch.isfinite(out[:, :, :64]))
+        got = torch.from_numpy(c.device_bytes()[0].copy()).view(TORCH[dtype]).view(4, 16, 128)[0, :3, 64:]
+        assert torch.equal(got, k[:, 64:].cpu())
+
+
 def test_rows_of_zeros_and_of_infinities():
     """A zero row norms to zero (eps keeps it finite); an infinite element spoils its own head only."""
     cache = Cache(2, 1, 16, 64, "float16", seed=19)

@@ -92,7 +92,7 @@ class Batch:
         call(kv.lib.kvfx_decode_shared, *self.args(out, **kw))
         return out.cpu()
 
-    def check(self, got, lens=None, rows=None):
+    def check(self, got, lens=None, rows=None, adds=None):
         lens = self.lens if lens is None else lens
         for r, n in enumerate(lens):
             if rows is not None and r not in rows:
@@ -106,13 +106,19 @@ class Batch:
             q = self.q[r].double().view(self.heads, -1, self.hd)
             p = torch.softmax(q @ k.transpose(1, 2) / math.sqrt(self.hd), -1)
             want, weight = p @ v, p @ v.abs()
-            a = (q.abs() @ k.abs().transpose(1, 2)).amax(-1, keepdim=True) / math.sqrt(self.hd)
+            seen = torch.where(k.abs() > 1e30, 0.0, k.abs())  # (scores past FP32's lowest value weigh exactly 0)
+            a = (q.abs() @ seen.transpose(1, 2)).amax(-1, keepdim=True) / math.sqrt(self.hd)
             split = 0.0 if self.dtype == "float32" else 2.0**-18
-            tol = weight * (2 * a * (split + self.hd * 2.0**-23) + split + 2.0**-21 + n * 2.0**-23)
+            tol = weight * (2 * a * (split + self.hd * 2.0**-23) + split + 2.0**-21 + (adds or n) * 2.0**-23)
             if self.dtype == "float16":
                 tol = tol + n * 2.0**-25 * v.abs().max()
             err = (got[r].double().view(self.heads, -1, self.hd) - want).abs()
             assert torch.all(err <= tol), (r, n, float((err / tol).max()))
+
+
+    def poison(self, key, pages, heads=slice(None)):
+        self.k[pages, heads] = key
+        self.dk.copy_(self.k)
 
 
 CASES = [  # groups (rows, prefix), lens, heads, q_group, hd, bs, dtype
@@ -167,6 +173,69 @@ def test_large_and_growing_scores(dtype, hd):
     b = Batch(groups, lens, 2, 4, hd, dtype=dtype, k_drift=0.125)
     b.check(b.run())
     assert kv.device_status(0) == 0
+
+
+# One launch, row by row; tails that join the prefix's pieces; a merge of several splits.
+FORMS = [([(3, 64)], [64, 80, 100], 0), ([(4, 800)], [800, 816, 1000, 1056], 0), ([(3, 320)], [320, 336, 900], 1000)]
+
+
+@pytest.mark.parametrize("groups,lens,room", FORMS)
+def test_scores_of_nan_come_through(groups, lens, room):
+    b = Batch(groups, lens, 2, 4, 128, room=room)
+    shared = [int(x) for x in b.table[0, : groups[0][1] // 16]]
+    b.poison(float("nan"), shared, 0)  # every score of the prefix, in one of two heads
+    got = b.run().view(len(lens), 2, 4, 128)
+    assert torch.all(torch.isnan(got[:, 0])) and torch.all(torch.isfinite(got[:, 1]))
+    b = Batch(groups, lens, 2, 4, 128, room=room)
+    b.poison(float("nan"), int(b.table[1, groups[0][1] // 16]), 1)  # the second row's first page of its own
+    got = b.run().view(len(lens), 2, 4, 128)
+    assert torch.all(torch.isnan(got[1, 1])) and torch.all(torch.isfinite(got[1, 0]))
+    assert torch.all(torch.isfinite(got[[0, 2]]))
+    assert kv.device_status(0) == 0
+
+
+@pytest.mark.parametrize("where", ["first page", "prefix", "own pages"])
+@pytest.mark.parametrize("groups,lens,room", FORMS)
+def test_scores_below_the_lowest_value_weigh_nothing(groups, lens, room, where):
+    # -2e38 x 4 a dimension sums past FP32's range: the score is -inf, its weight 0.
+    b = Batch(groups, lens, 2, 4, 128, room=room)
+    pre = groups[0][1] // 16
+    b.q.fill_(4.0)
+    b.dq.copy_(b.q)
+    rows = range(len(lens))
+    if where == "first page":
+        pages = [int(b.table[0, 0])]
+    elif where == "prefix":
+        pages, rows = [int(x) for x in b.table[0, :pre]], [r for r in rows if lens[r] > groups[0][1]]
+    else:
+        pages = sorted({int(b.table[r, j]) for r in rows for j in range(pre, -(-lens[r] // 16))})
+    b.poison(-2e38, pages)
+    b.check(b.run(), rows=rows)
+    assert kv.device_status(0) == 0
+
+
+@pytest.mark.parametrize("pages", [1 << 18, 1 << 19])
+def test_prefixes_of_more_tiles_than_a_block_joins(pages):
+    # A few pages over and over: the attention of those few, which is what it
+    # is compared with. A group ahead moves the runs off the prefix's first tile.
+    distinct, hd, bs = 64, 64, 16
+    b = Batch([(1, 8 * bs), (2, distinct * bs)], [8 * bs, distinct * bs, distinct * bs], 1, 4, hd)
+    width = pages + 2
+    table = np.zeros((3, width), np.uint64)
+    table[0, : pages - 8] = np.tile(b.table[0, :8], pages // 8 - 1)
+    table[1:, :pages] = np.tile(b.table[1, :distinct], pages // distinct)
+    sizes = [(pages - 8) * bs, pages * bs]
+    lens, groups = np.array([sizes[0], sizes[1], sizes[1]], np.uint64), (kv.KvfxPrefixGroup * 2)((1, sizes[0]), (2, sizes[1]))
+    reach = pages * bs + 16
+    need = kv.lib.kvfx_decode_shared_workspace_bytes(ctypes.byref(b.cache), groups, 2, 4, reach)
+    out, ws = torch.full((3, 4, hd), 7.0, device="cuda"), torch.empty(need, dtype=torch.uint8, device="cuda")
+    call(kv.lib.kvfx_decode_shared, ctypes.byref(b.cache), b.dq, out, u64(table), u64(lens), groups, 2, width, 4, reach, ws, need, None)
+    torch.cuda.synchronize()
+    assert kv.device_status(0) == 0
+    # One accumulator takes at most 8 tiles of 128 tokens before a sum that rounds takes it: 1024 truncated
+    # additions, then half a unit each for a run's 32 of those and the runs' join (at most 258), and for the
+    # weights' sum (7 levels within a tile, 256 tiles, the join): 1024 + (32 + 258 + 7 + 256 + 258) / 2.
+    b.check(out.cpu(), adds=1430)
 
 
 @pytest.mark.parametrize("room", [0, 1000])
