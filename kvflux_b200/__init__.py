@@ -9,7 +9,10 @@ Two native surfaces, both built in-tree by ``python kvflux_b200/build.py``:
   read_paged_kv, paged_attention, paged_attention_batch, append_token_cow,
   PrefixCache, SequenceLifecycle, ...) running on those kernels, plus
   BatchDecodeSession (batched decode steps over a device-resident block table)
-  and write_paged_kv_layers / read_paged_kv_layers (one launch for all layers).
+  and write_paged_kv_layers / read_paged_kv_layers (one launch for all layers),
+  paged_attention_batch_shared (requests that share a prompt's pages),
+  fork_sequence / compact_sequence (children, evictions), and RotaryTable /
+  write_paged_kv_rotated (norms and rotary positions of new tokens).
 
 There is no fallback: importing fails loudly if the extension is not built.
 """
