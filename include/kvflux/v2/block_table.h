@@ -51,6 +51,10 @@ public:
     // cache miss each.
     void copy_ids(PhysicalBlockID* out, std::size_t first = 0) const;
 
+    // How many of the first `limit` entries are `other`'s, page for page: the
+    // length of their common beginning. Looks no page up in the pool.
+    std::size_t common_entries(const BlockTable& other, std::size_t limit) const noexcept;
+
     // Change tracking (see the file comment). Stamps come from one
     // process-wide counter, so equal values always mean the same contents.
     std::uint64_t lineage() const noexcept { return lineage_; }
@@ -75,6 +79,8 @@ public:
     void clear() noexcept;
 
 private:
+    // Room for one more entry.
+    void make_room();
     // Records an edit of entries from `index` on (not an append).
     void edited(std::size_t index) noexcept;
 

@@ -11,7 +11,9 @@
 // ring of the last kEdits edits.
 #include "kvflux/v2/block_table.h"
 
+#include <algorithm>
 #include <atomic>
+#include <cstring>
 #include <stdexcept>
 #include <utility>
 
@@ -79,14 +81,31 @@ std::size_t BlockTable::first_changed_since(std::uint64_t revision) const noexce
     return low;
 }
 
+std::size_t BlockTable::common_entries(const BlockTable& other, std::size_t limit) const noexcept {
+    // Runs of 32 entries compared as bytes (a handle has no padding), then the
+    // run that differs entry by entry.
+    static_assert(sizeof(PhysicalBlockHandle) == sizeof(std::size_t) + sizeof(std::uint64_t));
+    constexpr std::size_t kRun = 32;
+    const std::size_t n = std::min({limit, entries_.size(), other.entries_.size()});
+    std::size_t i = 0;
+    while (i + kRun <= n && std::memcmp(&entries_[i], &other.entries_[i], kRun * sizeof(PhysicalBlockHandle)) == 0) i += kRun;
+    while (i < n && entries_[i] == other.entries_[i]) ++i;
+    return i;
+}
+
 PhysicalBlockPool& BlockTable::pool() const {
     if (pool_ == nullptr) throw std::logic_error("block table was moved from");
     return *pool_;
 }
 
+// Doubles: a table grown page by page copies each entry a constant number of times.
+void BlockTable::make_room() {
+    if (entries_.size() == entries_.capacity()) entries_.reserve(std::max<std::size_t>(8, 2 * entries_.size()));
+}
+
 PhysicalBlockID BlockTable::append_new() {
     PhysicalBlockPool& p = pool();
-    entries_.reserve(entries_.size() + 1);  // the push below cannot throw
+    make_room();  // the push below cannot throw
     const PhysicalBlockHandle h = p.allocate();
     entries_.push_back(h);
     return h.id;
@@ -94,7 +113,7 @@ PhysicalBlockID BlockTable::append_new() {
 
 void BlockTable::append_existing(PhysicalBlockHandle h) {
     PhysicalBlockPool& p = pool();
-    entries_.reserve(entries_.size() + 1);
+    make_room();
     p.retain(h);
     entries_.push_back(h);
 }

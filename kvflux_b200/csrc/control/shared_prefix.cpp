@@ -23,11 +23,7 @@ std::vector<PrefixGroup> plan_shared_prefixes(const std::vector<const SequenceSt
         }
     }
     const std::size_t block = sequences.front()->block_size();
-    auto read = [](const SequenceState& s, std::vector<PhysicalBlockID>& ids) {
-        ids.resize(s.num_allocated_blocks());
-        if (!ids.empty()) s.copy_physical_block_ids(ids.data());
-        ids.resize(s.num_tokens() / s.block_size());  // whole pages only
-    };
+    auto whole_pages = [](const SequenceState& s) { return s.num_tokens() / s.block_size(); };
     auto close = [&](std::size_t rows, std::size_t pages) {
         if (pages < kMinSharedPages || rows < 2) pages = 0;
         if (pages == 0 && !groups.empty() && groups.back().prefix_tokens == 0) {
@@ -36,15 +32,11 @@ std::vector<PrefixGroup> plan_shared_prefixes(const std::vector<const SequenceSt
             groups.push_back({rows, pages * block});
         }
     };
-    std::vector<PhysicalBlockID> last, next;
-    read(*sequences.front(), last);
-    std::size_t rows = 1, shared = last.size();
+    std::size_t rows = 1, shared = whole_pages(*sequences.front());
     for (std::size_t r = 1; r < sequences.size(); ++r) {
-        read(*sequences[r], next);
-        const std::size_t both = std::min(last.size(), next.size());
-        const auto differ = std::mismatch(last.begin(), last.begin() + static_cast<std::ptrdiff_t>(both), next.begin());
+        const SequenceState &last = *sequences[r - 1], &next = *sequences[r];
         const std::size_t common =
-            std::min(shared, static_cast<std::size_t>(differ.first - last.begin()));
+            last.block_table().common_entries(next.block_table(), std::min(shared, whole_pages(next)));
         // Saved page reads with this sequence, and without it.
         if (common >= kMinSharedPages && rows * common >= (rows - 1) * shared) {
             ++rows;
@@ -52,9 +44,8 @@ std::vector<PrefixGroup> plan_shared_prefixes(const std::vector<const SequenceSt
         } else {
             close(rows, shared);
             rows = 1;
-            shared = next.size();
+            shared = whole_pages(next);
         }
-        last.swap(next);
     }
     close(rows, shared);
     return groups;

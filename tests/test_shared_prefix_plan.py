@@ -98,3 +98,11 @@ def test_fork_prefix_shares_and_returns_pages():
     assert p.available() == 5 and c.physical_block_id(5) != src.physical_block_id(5)
     c.move_from(src.fork_prefix(3, 0))
     assert c.num_tokens() == 0 and p.available() == 6 and src.block_table().ref_count(0) == 1
+
+
+@pytest.mark.parametrize("pages", [31, 32, 33, 63, 64, 65, 100])
+def test_common_pages_end_at_any_entry(pages):
+    p = pool()
+    src = grown(p, 1, 120 * 16)
+    assert plan([src] + children(src, pages, [900, 900])) == [(3, pages * 16)]
+    assert plan(children(src, pages, [900]) + [src]) == [(2, pages * 16)]
