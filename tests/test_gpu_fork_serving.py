@@ -5,9 +5,10 @@ prefix, an eviction, more steps) with every attention output checked in 64
 bits over what the cache holds.
 
 Attention tolerance: Q and the weights are pairs of 16-bit values, off by at
-most 2^-18 of themselves; with A = the row's largest sum |q_i k_i| / sqrt(hd),
-a score is off by at most A (2^-18 + hd 2^-23), which counts twice (weight and
-sum); 2^-18 + 2^-21 for weights and exponential, n 2^-23 for n additions; all
+most 2^-17 of themselves (bf16: unit 2^-7, low part up to 2^-8, whose unit is
+2^-16); with A = the row's largest sum |q_i k_i| / sqrt(hd),
+a score is off by at most A (2^-17 + hd 2^-23), which counts twice (weight and
+sum); 2^-17 + 2^-21 for weights and exponential, n 2^-23 for n additions; all
 against sum p |v|."""
 import math
 
@@ -48,7 +49,7 @@ def check_row(q, k, v, got):
     k, v = (x.double().permute(1, 0, 2) for x in (k, v))
     p = torch.softmax(q @ k.transpose(1, 2) / math.sqrt(HD), -1)
     a = (q.abs() @ k.abs().transpose(1, 2)).amax(-1, keepdim=True) / math.sqrt(HD)
-    tol = (p @ v.abs()) * (2 * a * (2.0**-18 + HD * 2.0**-23) + 2.0**-18 + 2.0**-21 + k.shape[1] * 2.0**-23)
+    tol = (p @ v.abs()) * (2 * a * (2.0**-17 + HD * 2.0**-23) + 2.0**-17 + 2.0**-21 + k.shape[1] * 2.0**-23)
     assert torch.all((got.double().view(KVH, -1, HD) - p @ v).abs() <= tol)
 
 

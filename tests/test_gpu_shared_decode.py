@@ -6,13 +6,13 @@ rows, refused rows, bad pages, large scores, shapes without a fast kernel,
 graph replay and two calls in flight.
 
 Tolerance, per output. Q and the softmax weights are pairs of 16-bit values:
-each is off by at most 2^-18 of itself (bf16: half a unit of the low part, whose
-size is at most half a unit of the high part; fp16's 2^-22 has a floor of 2^-25
+each is off by at most 2^-17 of itself (bf16, of x in [1, 2): the high part's unit
+is 2^-7, so the low part is at most 2^-8, with a unit of 2^-16 of which half is lost; fp16's 2^-22 has a floor of 2^-25
 for weights whose low part is below its smallest step). With A = the largest
 sum |q_i k_i| / sqrt(hd) of the row, a score is off by at most
-A (2^-18 + hd 2^-23), counting one truncation of an FP32 accumulator an
+A (2^-17 + hd 2^-23), counting one truncation of an FP32 accumulator an
 addend; that is each weight's relative error, and the sum's, so it counts
-twice. Weights add 2^-18 and 2^-21 for the exponential and the joins, the
+twice. Weights add 2^-17 and 2^-21 for the exponential and the joins, the
 accumulation of n addends n 2^-23. All count against W = sum p |v|."""
 import ctypes
 import math
@@ -108,7 +108,7 @@ class Batch:
             want, weight = p @ v, p @ v.abs()
             seen = torch.where(k.abs() > 1e30, 0.0, k.abs())  # (scores past FP32's lowest value weigh exactly 0)
             a = (q.abs() @ seen.transpose(1, 2)).amax(-1, keepdim=True) / math.sqrt(self.hd)
-            split = 0.0 if self.dtype == "float32" else 2.0**-18
+            split = 0.0 if self.dtype == "float32" else 2.0**-17
             tol = weight * (2 * a * (split + self.hd * 2.0**-23) + split + 2.0**-21 + (adds or n) * 2.0**-23)
             if self.dtype == "float16":
                 tol = tol + n * 2.0**-25 * v.abs().max()
