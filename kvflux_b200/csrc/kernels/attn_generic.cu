@@ -10,7 +10,8 @@
 // Semantics follow the reference (KVFlux src/v2/paged_attention.cu:74-153):
 // KV head = q_head / (q_heads / kv_heads); a single sequence's query i sees
 // positions <= kv_tokens - query_tokens + i; a batch row sees all
-// sequence_lengths[r] positions.
+// sequence_lengths[r] positions. The rows of kvfx_decode_shared keep its
+// contract: bounds by group, rows of length 0 left alone.
 #include <algorithm>
 #include <cmath>
 
@@ -21,6 +22,15 @@ namespace kvfx {
 namespace {
 
 constexpr int kWarps = 4;
+
+// kvfx_decode_shared's groups (n = 0 for the other entry points): group g holds
+// rows [row_end[g - 1], row_end[g]), which share prefix[g] tokens.
+struct RowGroups {
+    uint32_t n;
+    uint32_t row_end[KVFX_MAX_PREFIX_GROUPS];
+    uint64_t prefix[KVFX_MAX_PREFIX_GROUPS];
+    uint64_t max_len;
+};
 
 struct GenericParams {
     const float* q;
@@ -35,12 +45,12 @@ struct GenericParams {
     uint64_t num_blocks;
     uint32_t q_heads, kv_heads, bs, hd;
     float qscale;
-    bool skip_empty;
     unsigned* status;
+    RowGroups groups;
 };
 
 template <typename T, int NV>
-__global__ void __launch_bounds__(kWarps * 32) attn_generic_kernel(const GenericParams p) {
+__global__ void __launch_bounds__(kWarps * 32) attn_generic_kernel(const __grid_constant__ GenericParams p) {
     extern __shared__ float q_s[];  // [kWarps][hd]
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     const uint64_t row_id = static_cast<uint64_t>(blockIdx.x) * kWarps + warp;
@@ -54,8 +64,14 @@ __global__ void __launch_bounds__(kWarps * 32) attn_generic_kernel(const Generic
     if (p.lens != nullptr) {
         visible = p.lens[u];
         brow = p.blocks + u * p.row_stride;
-        if (visible == 0 && p.skip_empty) return;
-        if (visible == 0 || visible > p.row_stride * p.bs) {  // outside the table row: refuse
+        bool outside = visible == 0 || visible > p.row_stride * p.bs;  // of the table row
+        if (p.groups.n != 0) {
+            if (visible == 0) return;
+            uint32_t g = 0;
+            while (u >= p.groups.row_end[g]) ++g;
+            outside = outside || visible < p.groups.prefix[g] || visible > p.groups.max_len;
+        }
+        if (outside) {  // refuse
             if (lane == 0) raise_flag(p.status, KVFX_FLAG_BAD_INDEX);
             return;
         }
@@ -173,8 +189,16 @@ cudaError_t launch_attention_generic(const CacheView& c, const GenericAttnArgs& 
     p.bs = c.bs;
     p.hd = c.hd;
     p.qscale = static_cast<float>(1.4426950408889634 / std::sqrt(static_cast<double>(c.hd)));
-    p.skip_empty = a.skip_empty;
     p.status = status;
+    if (a.num_groups > KVFX_MAX_PREFIX_GROUPS) return cudaErrorInvalidValue;
+    p.groups.n = a.num_groups;
+    p.groups.max_len = a.max_len;
+    uint64_t rows = 0;
+    for (uint32_t g = 0; g < a.num_groups; ++g) {
+        rows += a.groups[g].rows;
+        p.groups.row_end[g] = static_cast<uint32_t>(rows);
+        p.groups.prefix[g] = a.groups[g].prefix_tokens;
+    }
     switch (c.dtype) {
     case KVFX_F16: return launch_t<__half>(p, s);
     case KVFX_BF16: return launch_t<__nv_bfloat16>(p, s);

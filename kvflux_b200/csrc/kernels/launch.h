@@ -274,7 +274,12 @@ struct GenericAttnArgs {
     uint64_t units;             // batch size, or query_tokens for a single sequence
     uint64_t kv_tokens;         // single-sequence mode: sequence length
     uint32_t q_heads;
-    bool skip_empty = false;    // batch mode: a length of 0 is a padding row, not an error
+    // Batch mode of kvfx_decode_shared: the rows' groups (null otherwise) and
+    // the bound of their lengths. A length of 0 is then a padding row, and one
+    // outside [its group's prefix, max_len] is refused.
+    const kvfx_prefix_group* groups = nullptr;
+    uint32_t num_groups = 0;
+    uint64_t max_len = 0;
 };
 cudaError_t launch_attention_generic(const CacheView& c, const GenericAttnArgs& a,
                                      unsigned* status, cudaStream_t s);

@@ -271,7 +271,9 @@ cudaError_t launch_decode_shared(const CacheView& c, const SharedArgs& a, unsign
         uint64_t rows = 0;
         for (uint32_t g = 0; g < a.num_groups; ++g) rows += a.groups[g].rows;
         GenericAttnArgs g{a.q, a.o, a.table, a.max_blocks, a.lens, rows, 0, a.q_heads};
-        g.skip_empty = true;
+        g.groups = a.groups;
+        g.num_groups = a.num_groups;
+        g.max_len = a.max_len;
         return launch_attention_generic(c, g, status, s);
     }
     cudaError_t err = cudaSuccess;
