@@ -264,7 +264,7 @@ int kvfx_decode(const kvfx_cache* cache, const float* q, float* o,
  * 128 and block_size 16, with 16-byte aligned bases, q and o, read the prefix on
  * the tensor cores (at the FP32-class accuracy of the other attention entry
  * points), unless the rows are so short that reading them one by one is
- * faster; other shapes run row by row, each reading its whole table row.
+ * faster; other shapes run row by row, each reading all of its pages.
  * No counterpart in the reference, whose batch attention re-reads shared pages
  * for every row (src/v2/paged_attention.cu:248-313).
  */

@@ -11,7 +11,8 @@
 // KV head = q_head / (q_heads / kv_heads); a single sequence's query i sees
 // positions <= kv_tokens - query_tokens + i; a batch row sees all
 // sequence_lengths[r] positions. The rows of kvfx_decode_shared keep its
-// contract: bounds by group, rows of length 0 left alone.
+// contract: bounds by group, rows of length 0 left alone, the prefix's pages
+// taken from the group's first row.
 #include <algorithm>
 #include <cmath>
 
@@ -61,15 +62,19 @@ __global__ void __launch_bounds__(kWarps * 32) attn_generic_kernel(const __grid_
 
     uint64_t visible;
     const uint64_t* brow;
+    const uint64_t* prefix_row;  // names the positions below prefix
+    uint64_t prefix = 0;
     if (p.lens != nullptr) {
         visible = p.lens[u];
-        brow = p.blocks + u * p.row_stride;
+        brow = prefix_row = p.blocks + u * p.row_stride;
         bool outside = visible == 0 || visible > p.row_stride * p.bs;  // of the table row
         if (p.groups.n != 0) {
             if (visible == 0) return;
             uint32_t g = 0;
             while (u >= p.groups.row_end[g]) ++g;
-            outside = outside || visible < p.groups.prefix[g] || visible > p.groups.max_len;
+            prefix = p.groups.prefix[g];
+            prefix_row = p.blocks + (g == 0 ? 0 : p.groups.row_end[g - 1]) * p.row_stride;
+            outside = outside || visible < prefix || visible > p.groups.max_len;
         }
         if (outside) {  // refuse
             if (lane == 0) raise_flag(p.status, KVFX_FLAG_BAD_INDEX);
@@ -77,7 +82,7 @@ __global__ void __launch_bounds__(kWarps * 32) attn_generic_kernel(const __grid_
         }
     } else {
         visible = p.kv_tokens - p.units + u + 1;
-        brow = p.blocks;
+        brow = prefix_row = p.blocks;
     }
     const T* kc = reinterpret_cast<const T*>(p.k_cache);
     const T* vc = reinterpret_cast<const T*>(p.v_cache);
@@ -98,7 +103,7 @@ __global__ void __launch_bounds__(kWarps * 32) attn_generic_kernel(const __grid_
         uint64_t rowoff = 0;
         if (t < visible) {
             const uint64_t lb = t / p.bs;
-            uint64_t blk = __ldg(brow + lb);
+            uint64_t blk = __ldg((t < prefix ? prefix_row : brow) + lb);
             if (blk >= p.num_blocks) {
                 raise_flag(p.status, KVFX_FLAG_BAD_INDEX);
                 blk = 0;

@@ -71,3 +71,17 @@ def test_every_group_has_its_own_bound(shape):
     assert kv.device_status(0) == kv.KVFX_FLAG_BAD_INDEX
     b.check(got, lens=[64, 100, 1, 320, 333], rows=[1, 2, 4])
     assert torch.all(got[[0, 3]] == 7.0)
+
+
+@pytest.mark.parametrize("first", [300, 0])
+@pytest.mark.parametrize("shape", SHAPES)
+def test_only_the_first_row_names_the_prefix(shape, first):
+    """The other rows' entries for it are not read; the first row's are, also where that row is padding."""
+    lens = [first, 270, 256, 70, 64]
+    b = batch(shape, [(3, 256), (2, 64)], lens)
+    table = b.table.copy()
+    table[1:3, : 256 // b.bs] = b.pages + 5
+    table[4, : 64 // b.bs] = b.pages + 5
+    b.dtable = u64(table)
+    b.check(b.run())
+    assert kv.device_status(0) == 0

@@ -1,0 +1,54 @@
+"""Weights far below a row's largest one, in fp16 caches: many tokens of
+weight near 2^-26 behind one of weight 1 in every page, whose own value is 0,
+so that the output is what the small weights carry.
+
+Tolerance. A weight is a pair of fp16 values: off by at most 2^-22 of itself
+(test_gpu_shared_decode's bound, which covers scores, exponential and
+additions too), or, below fp16's smallest step 2^-24, by half of that step.
+The weights enter the products times 2^7 (relative to a row's running maximum,
+which the largest score passes by 2^8 at most), so half a step is at most
+2^-32 of the largest weight: 2^-32 / L a small token, with L the sum of a
+row's weights relative to the largest, against small weights of 2^-25.97 / L:
+2^-6 of the output."""
+import math
+
+import numpy as np
+import pytest
+import torch
+
+import kvflux_b200 as kv
+from test_gpu_shared_decode import FORMS, Batch
+
+pytestmark = pytest.mark.gpu
+
+HD = 64
+KEY = 2.25  # score 64 * 2.25 / 8 = 18, 25.97 in base 2
+
+
+def small_weights(groups, lens, room, group):
+    b = Batch(groups, lens, 2, group, HD, dtype="float16", room=room)
+    live = ~torch.isnan(b.k)
+    b.k[live], b.v[live] = 0.0, 1.0
+    first = live[:, :, 0, 0]
+    b.k[:, :, 0][first] = KEY
+    b.v[:, :, 0][first] = 0.0
+    b.q.fill_(1.0)
+    for d, h in ((b.dk, b.k), (b.dv, b.v), (b.dq, b.q)):
+        d.copy_(h)
+    return b
+
+
+@pytest.mark.parametrize("group", [4, 9])
+@pytest.mark.parametrize("groups,lens,room", FORMS + [([(40, 2064)], [2064 + 3 * i for i in range(40)], 0)])
+def test_small_weights_count(cuda, groups, lens, room, group):
+    kv.device_status(0, clear=True)
+    b = small_weights(groups, lens, room, group)
+    got = b.run().double()
+    assert kv.device_status(0) == 0
+    weight = math.exp(-HD * KEY / math.sqrt(HD))
+    for r, n in enumerate(lens):
+        large = -(-n // 16)
+        want = (n - large) * weight / (large + (n - large) * weight)
+        a = HD * KEY / math.sqrt(HD)
+        tol = want * (2.0**-6 + 2 * a * (2.0**-22 + HD * 2.0**-23) + 2.0**-22 + 2.0**-21 + n * 2.0**-23)
+        assert float((got[r] - want).abs().max()) <= tol, (r, n, float(got[r].min()), float(got[r].max()), want)
