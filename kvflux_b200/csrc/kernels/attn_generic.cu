@@ -118,8 +118,9 @@ __global__ void __launch_bounds__(kWarps * 32) attn_generic_kernel(const __grid_
 #pragma unroll
         for (int x = 16; x > 0; x >>= 1) cm = fmaxf(cm, __shfl_xor_sync(0xffffffffu, cm, x));
         const float m_new = fmaxf(m, cm);
-        const float alpha = exp2f(m - m_new);
-        const float pw = exp2f(s - m_new);
+        const float m_sub = m_new == -INFINITY ? 0.f : m_new;  // scores of -inf so far: weights of 0
+        const float alpha = exp2f(m - m_sub);
+        const float pw = exp2f(s - m_sub);
         float ps = pw;
 #pragma unroll
         for (int x = 16; x > 0; x >>= 1) ps += __shfl_xor_sync(0xffffffffu, ps, x);

@@ -85,3 +85,24 @@ def test_only_the_first_row_names_the_prefix(shape, first):
     b.dtable = u64(table)
     b.check(b.run())
     assert kv.device_status(0) == 0
+
+
+@pytest.mark.parametrize("tokens", [32, 256])
+@pytest.mark.parametrize("shape", [s for s in SHAPES if s[0] != "float16"])  # fp16 holds no such keys
+def test_scores_below_the_lowest_value_weigh_nothing(shape, tokens):
+    """-2e38 x 4 a dimension sums past FP32's range: such a score is -inf, its weight 0, wherever it stands."""
+    b = batch(shape, [(3, 256)], [300, 270, 257])
+    b.q.fill_(4.0)
+    b.dq.copy_(b.q)
+    b.poison(-2e38, [int(x) for x in b.table[0, : tokens // b.bs]])
+    b.check(b.run())
+    assert kv.device_status(0) == 0
+
+
+@pytest.mark.parametrize("shape", SHAPES)
+def test_scores_of_nan_come_through(shape):
+    b = batch(shape, [(3, 256)], [300, 270, 257])
+    b.poison(float("nan"), [int(x) for x in b.table[0, : 32 // b.bs]], 0)  # the first 32 scores, in one of two heads
+    got = b.run().view(3, 2, 4, b.hd)
+    assert torch.all(torch.isnan(got[:, 0])) and torch.all(torch.isfinite(got[:, 1]))
+    assert kv.device_status(0) == 0
