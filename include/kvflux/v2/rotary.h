@@ -61,8 +61,9 @@ struct ProjectedTokens {
 // on the legacy default stream; an empty mapping returns at once. Throws
 // invalid_argument for null or foreign-device pointers, a table of another
 // device or wider than the head, strides below a token's heads, a position
-// count other than the slots', and query_out_device overlapping an input or
-// the cache; out_of_range for a slot or position out of range.
+// count other than the slots', an input (norm weights among them) in the
+// cache, and query_out_device overlapping an input or the cache; out_of_range
+// for a slot or position out of range.
 void write_paged_kv_rotated(PagedKVStorage& storage, const RotaryTable& table, const HeadNorms& norms,
                             const ProjectedTokens& tokens, std::size_t query_heads,
                             const std::vector<std::size_t>& positions, const SlotMapping& slot_mapping,

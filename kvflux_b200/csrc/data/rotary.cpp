@@ -1,6 +1,8 @@
 // RotaryTable and write_paged_kv_rotated (include/kvflux/v2/rotary.h).
 #include "kvflux/v2/rotary.h"
 
+#include <utility>
+
 #include "runtime.h"
 
 namespace kvflux::v2 {
@@ -86,12 +88,28 @@ void write_paged_kv_rotated(PagedKVStorage& storage, const RotaryTable& table, c
     if (query_heads != 0) {
         detail::require_device_pointer(tokens.query, storage.device(), "Q");
         detail::require_device_pointer(query_out_device, storage.device(), "Q output");
-        if (detail::overlaps(query_out_device, out_bytes, tokens.query, q_bytes) ||
-            detail::overlaps(query_out_device, out_bytes, tokens.key, k_bytes) ||
-            detail::overlaps(query_out_device, out_bytes, tokens.value, v_bytes) ||
-            detail::overlaps(query_out_device, out_bytes, storage.key_base(), layout.total_bytes())) {
+    }
+    // Nothing that is read may lie where the call writes.
+    const std::size_t weight_bytes = layout.head_size() * sizeof(float);
+    const std::pair<const void*, std::size_t> inputs[] = {
+        {tokens.key, k_bytes},
+        {tokens.value, v_bytes},
+        {tokens.query, q_bytes},
+        {norms.query_weight, norms.query_weight != nullptr ? weight_bytes : 0},
+        {norms.key_weight, norms.key_weight != nullptr ? weight_bytes : 0},
+        {table.device_table(), table.max_positions() * table.rotary_dim() * sizeof(float)},
+    };
+    for (const auto& [input, input_bytes] : inputs) {
+        if (input_bytes == 0) continue;
+        if (detail::overlaps(input, input_bytes, storage.key_base(), layout.total_bytes())) {
+            throw std::invalid_argument("rotated KV write inputs must not lie in the KV cache");
+        }
+        if (out_bytes != 0 && detail::overlaps(query_out_device, out_bytes, input, input_bytes)) {
             throw std::invalid_argument("Q output must not overlap the inputs or the KV cache");
         }
+    }
+    if (out_bytes != 0 && detail::overlaps(query_out_device, out_bytes, storage.key_base(), layout.total_bytes())) {
+        throw std::invalid_argument("Q output must not overlap the inputs or the KV cache");
     }
     const std::size_t bytes[2] = {n * sizeof(PhysicalSlot), n * sizeof(std::size_t)};
     const void* host[2] = {slot_mapping.data(), positions.data()};
