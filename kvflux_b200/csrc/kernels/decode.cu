@@ -394,9 +394,13 @@ decode_mma_kernel(const __grid_constant__ DecodeParams p, const __grid_constant_
         }
         mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 1));
         mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 2));
-        const bool need = mx > m_run + 8.f;
+        // In tail mode m_run is the maximum less kWeightShift, and the piece's
+        // m is that; the difference is exact near the bound, where m_run + 15
+        // rounds once scores pass 2^24.
+        constexpr float kShift = kTail ? kWeightShift<T> : 0.f;
+        const bool need = kTail ? mx - m_run > 8.f + kShift : mx > m_run + 8.f;
         if (__any_sync(0xffffffffu, need)) {
-            const float m_new = need ? mx : m_run;
+            const float m_new = need ? mx - kShift : m_run;
             float alpha = exp2f(m_run - m_new);
             if constexpr (kTail) alpha = need ? alpha : 1.f;  // (both may be -inf)
             l_run *= alpha;

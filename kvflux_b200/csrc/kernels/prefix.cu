@@ -36,18 +36,19 @@
 // TMEM columns: S/P buffers 0 and 128; O 256; Q behind it (hi then lo halves).
 // Precision: Q and P are fed as two 16-bit operands each, hi = round(x) and
 // lo = round(x - hi): in bf16 off by at most 2^-17 of x (one bf16 operand alone
-// is off by up to 2^-8 of each weight), in fp16 by 2^-23. The tensor cores truncate each sum into the FP32
-// accumulator, a bias that grows with the number of additions (measured over
-// 110 tiles in one accumulator: 2.4e-5 of O), hence the sum over flushes,
-// which rounds. (Kept in registers it is code that runs out of a cold
-// instruction cache at every segment's end, 6 us more at 7 tiles a CTA; left
-// to the merge kernel, 16 tiles a piece, it is 60 MB more to write and read at
-// 256 rows x 64 heads.) A flush takes all of O into registers and lets the
-// next PV go before it adds: 208 us against 218 at 256 rows x 64 heads x 16384
-// tokens, 620 -> 660 TFLOP/s of attention (twice that executed), where a tile
-// is bounded by its chain: softmax 1.2 us, PV and QK 0.6 us each. O is
-// rescaled in TMEM only when a tile's row maximum passes the running one by
-// more than 8.
+// is off by up to 2^-8 of each weight), in fp16 by 2^-22 with an absolute floor
+// of 2^-25, which is why P enters times 2^7 there (kWeightShift). The tensor
+// cores truncate each sum into the FP32 accumulator, a bias that grows with the
+// number of additions (measured over 110 tiles in one accumulator: 2.4e-5 of
+// O), hence the sum over flushes, which rounds. (Kept in registers it is code
+// that runs out of a cold instruction cache at every segment's end, 6 us more
+// at 7 tiles a CTA; left to the merge kernel, 16 tiles a piece, it is 60 MB
+// more to write and read at 256 rows x 64 heads.) A flush takes all of O into
+// registers and lets the next PV go before it adds: 208 us against 218 at 256
+// rows x 64 heads x 16384 tokens, 620 -> 660 TFLOP/s of attention (twice that
+// executed), where a tile is bounded by its chain: softmax 1.2 us, PV and QK
+// 0.6 us each. O is rescaled in TMEM only when a tile's row maximum passes the
+// running one by more than 8.
 #include <algorithm>
 #include <atomic>
 #include <cmath>
@@ -438,8 +439,12 @@ prefix_tc_kernel(const __grid_constant__ PrefixParams p, const __grid_constant__
                     tc::reg_fence32(sc + 96);
                     mx = fmaxf(fmaxf(max32(sc), max32(sc + 32)), fmaxf(max32(sc + 64), max32(sc + 96)));
                 }
-                const bool need = mx > m_run + 8.f;  // m_run = -inf: at any finite maximum
-                const float alpha = need ? ex2_approx(m_run - mx) : 1.f;  // 0 at the first tile
+                // m_run is the maximum less kWeightShift (-inf: replaced by any
+                // finite one). The difference is exact near the bound, where
+                // m_run + 15 rounds once scores pass 2^24.
+                const bool need = mx - m_run > 8.f + kWeightShift<T>;
+                const float m_new = mx - kWeightShift<T>;
+                const float alpha = need ? ex2_approx(m_run - m_new) : 1.f;  // 0 at the first tile
                 l_run *= alpha;
                 if (in_flush != 0 && __any_sync(0xffffffffu, need)) {
                     // O holds the flush's earlier tiles once PV(t - 1)
@@ -456,7 +461,7 @@ prefix_tc_kernel(const __grid_constant__ PrefixParams p, const __grid_constant__
                         tc::st32(tO + cb, ov);
                     }
                 }
-                if (need) m_run = mx;
+                if (need) m_run = m_new;
                 // P over its own S columns: chunk of 32 tokens -> 16 columns
                 // of hi pairs, 16 of lo pairs. The scores are read again
                 // chunk by chunk, the next one's load under this one's math.
