@@ -265,6 +265,8 @@ int kvfx_decode(const kvfx_cache* cache, const float* q, float* o,
  * the tensor cores (at the FP32-class accuracy of the other attention entry
  * points), unless the rows are so short that reading them one by one is
  * faster; other shapes run row by row, each reading all of its pages.
+ * Where a wait inside a kernel runs out (KVFX_FLAG_TIMEOUT), the rows that
+ * depend on it become NaN or stay as they were.
  * No counterpart in the reference, whose batch attention re-reads shared pages
  * for every row (src/v2/paged_attention.cu:248-313).
  */
@@ -390,6 +392,18 @@ int kvfx_device_status(int device, uint32_t* flags, int clear);
  * kernels do not wait on barriers.
  */
 int kvfx_selftest_wait_timeout(int device);
+
+/*
+ * kvfx_decode_shared as it ends when every wait of its prefix kernel has run
+ * out, without the waits: that kernel's pieces are given up by the code that
+ * the waits' end reaches, and the rest of the call joins them. Rows behind a
+ * prefix become NaN, whatever the workspace held; rows without one, and calls
+ * that launch no prefix kernel, are computed as ever. No flag is raised.
+ */
+int kvfx_selftest_lost_prefix(const kvfx_cache* cache, const float* q, float* o, const uint64_t* block_table,
+                              const uint64_t* seq_lens, const kvfx_prefix_group* groups, uint32_t num_groups,
+                              uint64_t max_blocks_per_seq, uint32_t q_heads, uint64_t max_seq_len,
+                              void* workspace, uint64_t workspace_bytes, void* stream);
 
 /* Library version, e.g. "kvflux-b200 0.1.0 sm_100a". */
 const char* kvfx_version(void);

@@ -105,6 +105,7 @@ def _load():
     L.kvfx_decode_shared_workspace_bytes.argtypes = [C, G, u32, u32, u64]
     L.kvfx_decode_shared_workspace_bytes.restype = u64
     L.kvfx_decode_shared.argtypes = [C, vp, vp, vp, vp, G, u32, u64, u32, u64, vp, u64, vp]
+    L.kvfx_selftest_lost_prefix.argtypes = L.kvfx_decode_shared.argtypes
     L.kvfx_attention_workspace_bytes.argtypes = [C, u64, u64, u32]
     L.kvfx_attention_workspace_bytes.restype = u64
     L.kvfx_attention.argtypes = [C, vp, vp, vp, u64, u64, u32, vp, u64, vp]
@@ -127,7 +128,8 @@ KVFX_SYMBOLS = (
     "kvfx_decode_pages_per_split", "kvfx_decode", "kvfx_decode_append", "kvfx_decode_noalloc",
     "kvfx_decode_shared_workspace_bytes", "kvfx_decode_shared", "kvfx_attention_workspace_bytes",
     "kvfx_attention", "kvfx_attention_batch",
-    "kvfx_last_error", "kvfx_device_status", "kvfx_selftest_wait_timeout", "kvfx_version",
+    "kvfx_last_error", "kvfx_device_status", "kvfx_selftest_wait_timeout", "kvfx_selftest_lost_prefix",
+    "kvfx_version",
 )
 
 DTYPE_CODE = {"float16": KVFX_F16, "bfloat16": KVFX_BF16, "float32": KVFX_F32}

@@ -550,10 +550,12 @@ uint64_t kvfx_decode_shared_workspace_bytes(const kvfx_cache* cache, const kvfx_
     return kvfx::shared_workspace_bytes(c, groups, num_groups, q_heads, max_seq_len);
 }
 
-int kvfx_decode_shared(const kvfx_cache* cache, const float* q, float* o, const uint64_t* block_table,
-                       const uint64_t* seq_lens, const kvfx_prefix_group* groups, uint32_t num_groups,
-                       uint64_t max_blocks_per_seq, uint32_t q_heads, uint64_t max_seq_len, void* workspace,
-                       uint64_t workspace_bytes, void* stream) {
+namespace {
+
+int decode_shared(const kvfx_cache* cache, const float* q, float* o, const uint64_t* block_table,
+                  const uint64_t* seq_lens, const kvfx_prefix_group* groups, uint32_t num_groups,
+                  uint64_t max_blocks_per_seq, uint32_t q_heads, uint64_t max_seq_len, void* workspace,
+                  uint64_t workspace_bytes, bool lose_prefix, void* stream) {
     kvfx::CacheView c;
     if (int rc = make_view(cache, &c); rc != KVFX_OK) return rc;
     uint64_t batch = 0;
@@ -579,9 +581,27 @@ int kvfx_decode_shared(const kvfx_cache* cache, const float* q, float* o, const 
     DeviceScope scope(c.device);
     if (scope.error() != cudaSuccess) return cuda_fail("select device", scope.error());
     const kvfx::SharedArgs a{q, o, block_table, seq_lens, max_blocks_per_seq, max_seq_len, q_heads,
-                             groups, num_groups, workspace};
+                             groups, num_groups, workspace, lose_prefix};
     const cudaError_t e = kvfx::launch_decode_shared(c, a, status_word(c.device), static_cast<cudaStream_t>(stream));
     return e == cudaSuccess ? KVFX_OK : cuda_fail("shared-prefix decode launch", e);
+}
+
+}  // namespace
+
+int kvfx_decode_shared(const kvfx_cache* cache, const float* q, float* o, const uint64_t* block_table,
+                       const uint64_t* seq_lens, const kvfx_prefix_group* groups, uint32_t num_groups,
+                       uint64_t max_blocks_per_seq, uint32_t q_heads, uint64_t max_seq_len, void* workspace,
+                       uint64_t workspace_bytes, void* stream) {
+    return decode_shared(cache, q, o, block_table, seq_lens, groups, num_groups, max_blocks_per_seq, q_heads,
+                         max_seq_len, workspace, workspace_bytes, false, stream);
+}
+
+int kvfx_selftest_lost_prefix(const kvfx_cache* cache, const float* q, float* o, const uint64_t* block_table,
+                              const uint64_t* seq_lens, const kvfx_prefix_group* groups, uint32_t num_groups,
+                              uint64_t max_blocks_per_seq, uint32_t q_heads, uint64_t max_seq_len, void* workspace,
+                              uint64_t workspace_bytes, void* stream) {
+    return decode_shared(cache, q, o, block_table, seq_lens, groups, num_groups, max_blocks_per_seq, q_heads,
+                         max_seq_len, workspace, workspace_bytes, true, stream);
 }
 
 uint64_t kvfx_attention_workspace_bytes(const kvfx_cache* cache, uint64_t query_tokens, uint64_t kv_tokens,

@@ -587,7 +587,8 @@ decode_mma_kernel(const __grid_constant__ DecodeParams p, const __grid_constant_
     }
     if (tid < static_cast<int>(G)) {
         part[tid * (HD + 2) + HD] = failed ? -INFINITY : s_m[0][tid];
-        part[tid * (HD + 2) + HD + 1] = failed ? 0.f : s_l[0][tid];
+        // (The merge kernel makes the row NaN; this one's own join leaves the split out.)
+        part[tid * (HD + 2) + HD + 1] = !failed ? s_l[0][tid] : kTail ? __int_as_float(0x7fc00000) : 0.f;
     }
     if constexpr (kTail) {
         pdl_wait();

@@ -222,6 +222,7 @@ struct PrefixArgs {
     const PrefixGroups* groups;
     float* part_o;
     float* part_ml;
+    bool lose;  // self-test: no segment's O comes
 };
 cudaError_t launch_prefix_tc(const CacheView& c, const PrefixArgs& a, const CacheMaps& maps, unsigned* status,
                              cudaStream_t s);
@@ -237,6 +238,7 @@ struct SharedArgs {
     const kvfx_prefix_group* groups;
     uint32_t num_groups;
     void* workspace;
+    bool lose_prefix;  // self-test: as if every load of the prefix kernel had failed
 };
 uint64_t shared_workspace_bytes(const CacheView& c, const kvfx_prefix_group* groups, uint32_t num_groups,
                                 uint32_t q_heads, uint64_t max_len);

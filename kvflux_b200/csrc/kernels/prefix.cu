@@ -147,6 +147,22 @@ __device__ __forceinline__ void list_segments(const PrefixParams& p, Segment* li
     if (starts) list[at] = s;
 }
 
+// The pieces of segments whose O never came (a bounded wait ran out): no
+// weight, and a sum that makes the rows joined with them NaN, whatever an
+// earlier call left in the workspace. Thread r of 128 writes query row r.
+// (Inlined behind the loop that it follows: as a call it makes 16 rows behind
+// 2064 tokens 16.4 us instead of 16.2.)
+__device__ __forceinline__ void lose_segments(const PrefixParams& p, const Segment* list, uint32_t k, uint32_t n,
+                                              uint32_t r) {
+#pragma unroll 1
+    for (; k < n; ++k) {
+        if (r < list[k].m_rows) {
+            reinterpret_cast<float2*>(p.part_ml)[static_cast<uint64_t>(list[k].slot) * kBM + r] =
+                make_float2(-INFINITY, __int_as_float(0x7fc00000));
+        }
+    }
+}
+
 // Walks the list tile by tile: segment k, tile j of its pair, and the running
 // tile ordinal t that indexes rings and barriers.
 struct Cursor {
@@ -598,10 +614,11 @@ prefix_tc_kernel(const __grid_constant__ PrefixParams p, const __grid_constant__
         };
         pdl_wait();
         uint32_t flush = 0;
+        uint32_t done = 0;
         bool ok = true;
         stage_q(list[0]);
 #pragma unroll 1
-        for (uint32_t k = 0; ok && k < n_seg; ++k) {
+        for (uint32_t k = 0; k < n_seg; ++k) {
             const uint32_t slot = list[k].slot, m_rows = list[k].m_rows, j_end = list[k].j_end, j0 = list[k].j;
             const bool live = quarter * 32 < m_rows;
             float m_o = -INFINITY, l = 0.f;  // scale of the sum, row sum
@@ -654,7 +671,9 @@ prefix_tc_kernel(const __grid_constant__ PrefixParams p, const __grid_constant__
                     mbar_arrive(&o_free);
                 }
             }
-            if (ok && live) {
+            if (!ok) break;
+            ++done;
+            if (live) {
                 __syncwarp();
                 const uint64_t at = static_cast<uint64_t>(slot) * kBM + quarter * 32;
 #pragma unroll 1
@@ -671,6 +690,7 @@ prefix_tc_kernel(const __grid_constant__ PrefixParams p, const __grid_constant__
                 __syncwarp();
             }
         }
+        if (!ok) lose_segments(p, list, done, n_seg, r);
     }
 
     tc::fence_before_sync();
@@ -679,6 +699,19 @@ prefix_tc_kernel(const __grid_constant__ PrefixParams p, const __grid_constant__
         tc::fence_after_sync();
         tc::tmem_dealloc(tmem, kTmemCols);
     }
+}
+
+// In place of the prefix kernel: every segment lost (the self-test's launch).
+__global__ void __launch_bounds__(kThreads) lost_prefix_kernel(const __grid_constant__ PrefixParams p) {
+    __shared__ uint32_t warp_count[kThreads / 32];
+    __shared__ Segment list[kMaxRun];
+    list_segments(p, list, warp_count);
+    __syncthreads();
+    uint32_t n_seg = 0;
+    for (int w = 0; w < kThreads / 32; ++w) n_seg += warp_count[w];
+    pdl_wait();
+    pdl_allow_next();
+    if (threadIdx.x < kBM) lose_segments(p, list, 0, n_seg, threadIdx.x);
 }
 
 template <int HD, typename T>
@@ -722,6 +755,7 @@ cudaError_t launch_prefix_tc(const CacheView& c, const PrefixArgs& a, const Cach
     p.part_ml = a.part_ml;
     p.status = status;
     if (ceil_div(a.groups->tiles(), a.grid) > kMaxRun) return cudaErrorInvalidValue;
+    if (a.lose) return launch_dependent(lost_prefix_kernel, dim3(a.grid), dim3(kThreads), s, p);
     if (c.hd == 128) {
         return c.dtype == KVFX_BF16 ? launch_hd<128, __nv_bfloat16>(c, p, a.grid, maps, s)
                                     : launch_hd<128, __half>(c, p, a.grid, maps, s);

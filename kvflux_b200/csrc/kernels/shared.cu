@@ -284,7 +284,8 @@ cudaError_t launch_decode_shared(const CacheView& c, const SharedArgs& a, unsign
     float* part_ml = reinterpret_cast<float*>(ws + plan.off_ml);
     float* tail = reinterpret_cast<float*>(ws + plan.off_tail);
     if (plan.grid != 0) {
-        const PrefixArgs pa{a.q, a.table, a.max_blocks, a.q_heads, plan.grid, plan.stream, &plan.groups, part_o, part_ml};
+        const PrefixArgs pa{a.q, a.table, a.max_blocks, a.q_heads, plan.grid, plan.stream, &plan.groups, part_o, part_ml,
+                            a.lose_prefix};
         const CacheMaps* groups = prefix_maps(c, &err);
         if (groups == nullptr) return err != cudaSuccess ? err : cudaErrorInvalidValue;
         err = launch_prefix_tc(c, pa, *groups, status, s);
