@@ -389,7 +389,7 @@ __device__ __forceinline__ void split2(float x0, float x1, uint32_t& hi, uint32_
 
 // Softmax weights as pairs of T enter the products times 2^kWeightShift<T>,
 // with a running maximum that the largest score passes by at most 8. A bf16
-// pair is off by 2^-17 of any weight; an fp16 one by 2^-22 of it, or, where its
+// pair is off by 2^-17 of any weight; an fp16 one by 2^-23 of it, or, where its
 // low half is below fp16's smallest step, by half of that step, 2^-25: all of
 // a weight near 2^-25, of which a long row may have many. Times 2^7 (so up to
 // 2^15, the most that fits) the floor is 2^-32 of the running maximum's weight.

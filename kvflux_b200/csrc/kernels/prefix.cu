@@ -36,7 +36,7 @@
 // TMEM columns: S/P buffers 0 and 128; O 256; Q behind it (hi then lo halves).
 // Precision: Q and P are fed as two 16-bit operands each, hi = round(x) and
 // lo = round(x - hi): in bf16 off by at most 2^-17 of x (one bf16 operand alone
-// is off by up to 2^-8 of each weight), in fp16 by 2^-22 with an absolute floor
+// is off by up to 2^-8 of each weight), in fp16 by 2^-23 with an absolute floor
 // of 2^-25, which is why P enters times 2^7 there (kWeightShift). The tensor
 // cores truncate each sum into the FP32 accumulator, a bias that grows with the
 // number of additions (measured over 110 tiles in one accumulator: 2.4e-5 of

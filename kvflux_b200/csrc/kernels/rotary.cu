@@ -17,7 +17,8 @@
 // pass before is computed. The norm's sum and the rotation's partner dims
 // move by shuffles inside the group. B200, 8192 tokens of 32 + 8 + 8 heads of
 // 128 bf16: 49 us, 5.6 TB/s (57 us with 64 threads a CTA, 71 us with 128, 60 us
-// without the pass ahead); a decode step's 64 tokens: 3.6 us.
+// without the pass ahead); a decode step's 64 tokens: 3.6 us. In FP32 106 us,
+// 3.8 TB/s (spills, see kMinCtas), and 4.4 us.
 #include <algorithm>
 #include <cmath>
 
@@ -28,7 +29,9 @@ namespace kvfx {
 namespace {
 
 constexpr int kThreads = 32;      // one warp a CTA: many small ones hide the chain of loads a token has
-constexpr int kMinCtas = 18;      // per SM (112 registers)
+// CTAs per SM: 96 registers. 16-bit rows fit; the four FP32 kernels, whose rows
+// in flight are twice as wide, spill 140 to 208 bytes.
+constexpr int kMinCtas = 18;
 constexpr int kAnyThreads = 128;  // of the element-wise kernel
 constexpr int kEl = 8;            // elements per lane
 constexpr int kRows = 4;          // rows in flight per lane group, and as many behind them
@@ -46,7 +49,7 @@ struct RotatedParams {
     float* q_out;
     char* k_cache;
     char* v_cache;
-    uint64_t tokens, max_positions, slot_count;
+    uint64_t max_positions, slot_count;
     uint32_t q_heads, kv_heads, hd, bs, rotary_dim, interleaved;
     float eps, inv_hd;
     unsigned* status;
@@ -291,7 +294,9 @@ __global__ void __launch_bounds__(kThreads, kMinCtas) write_rotated_kernel(const
 }
 
 // Any head size, rotary_dim and alignment: one warp per row, element by
-// element; the partner element is read again (from L1).
+// element; the partner element is read again (from L1). Bounded by its
+// instructions, one element a lane: 8192 tokens of 32 + 8 + 8 bf16 heads of 96
+// 136 us, 1.5 TB/s; 64 tokens 4.8 us.
 template <typename T>
 __global__ void __launch_bounds__(kAnyThreads) write_rotated_any_kernel(const __grid_constant__ RotatedParams p) {
     pdl_allow_next();
@@ -445,7 +450,6 @@ cudaError_t launch_write_rotated(const CacheView& c, const kvfx_rotary& rotary, 
         p.positions = a.positions + i;
         p.slots = a.slots + i;
         p.q_out = a.q_out + i * a.q_heads * c.hd;
-        p.tokens = n;
         cudaError_t e;
         switch (c.dtype) {
         case KVFX_F16: e = launch_t<__half>(p, n, vec, sms, s); break;

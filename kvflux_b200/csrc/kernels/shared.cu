@@ -225,7 +225,15 @@ bool make_plan(const CacheView& c, const kvfx_prefix_group* groups, uint32_t n, 
         // 256 rows x 64 heads behind 16384 tokens 385 us against 410 with the
         // merge kernel, 64 rows x 32 heads behind 8 prompts 62 / 64. Few rows
         // of some length are better split (16 rows x 8 KV heads of up to 32
-        // pages: 18.5 fused, 16.5 split).
+        // pages: 18.5 fused, 16.5 split). The bound is the host's (the longest
+        // row less the shortest prefix), so rows of 64 pages can stand at its
+        // end, as those of the 8 prompts do. Rows that all are as long as it
+        // says, behind 4096 tokens, fused / split, at 64, 256, 512 and 1024
+        // pages: 40 rows x 8 KV heads 43 / 47, 117 / 117, 219 / 213 and 422 /
+        // 403 us; 64 rows 69 / 62, 205 / 175, 385 / 328 and 748 / 620 (512
+        // CTAs, a wave of 444 and a rest as long as the wave); 48 rows x 8 KV
+        // heads of 64 dims 46 / 54 at 128 pages, 132 / 142 at 512; 256 rows
+        // 1222 / 1233 at 512.
         const uint64_t ctas = rows * c.heads * ceil_div(q_group, 8);
         uint32_t pps = decode_pages_per_split(c, rows, q_heads, tail_pages * 16, 0);
         if (tail_pages <= 16 || (tail_pages <= 512 && ctas >= 2 * static_cast<uint64_t>(device_sm_count(c.device)))) {
@@ -267,7 +275,9 @@ cudaError_t launch_decode_shared(const CacheView& c, const SharedArgs& a, unsign
     const bool aligned = ((reinterpret_cast<uintptr_t>(a.q) | reinterpret_cast<uintptr_t>(a.o) |
                            reinterpret_cast<uintptr_t>(c.k) | reinterpret_cast<uintptr_t>(c.v)) & 15u) == 0;
     if (!make_plan(c, a.groups, a.num_groups, a.q_heads, a.max_len, &plan) || !aligned) {
-        // Row by row over the whole table.
+        // Row by row, each reading all of its pages, shared ones too, one warp
+        // a query head: 16 rows of 32 + 8 FP32 heads of 128 behind 2064 tokens
+        // 1.2 ms.
         uint64_t rows = 0;
         for (uint32_t g = 0; g < a.num_groups; ++g) rows += a.groups[g].rows;
         GenericAttnArgs g{a.q, a.o, a.table, a.max_blocks, a.lens, rows, 0, a.q_heads};

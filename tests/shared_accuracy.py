@@ -11,7 +11,7 @@ together. Sums that truncate, of 16 products at a time: a score's 2 hd / 16,
 each by at most 2^-23 of values of a few units, 2e-6 to 4e-6; those of O, at
 most 128 a sum (8 tiles of 128 tokens, or a warp's pages of a split), by half
 of 2^-23 on average, 7.6e-6. Together sqrt(6.2^2 + 4^2 + 7.6^2) = 10.6e-6,
-below BOUND = 2^-16 = 15.3e-6. fp16 pairs (2^-22) are off by the sums alone.
+below BOUND = 2^-16 = 15.3e-6. fp16 pairs (2^-23) are off by the sums alone.
 A single operand is off by up to 2^-8 (bf16) or 2^-11 (fp16) of itself, rms
 2.3e-3 and 2.8e-4 at a binade's lower end and about 0.7 of that over a binade:
 above the bound by 10 and more."""
