@@ -22,7 +22,9 @@ struct PrefixGroup {
 // long as the pages it saves reading ((rows - 1) x shared pages) do not
 // shrink; runs that would share fewer than 8 pages share none, and consecutive
 // ones of those are one group. Sequences that should share belong next to each
-// other. All sequences must be non-null and of one pool (invalid_argument).
+// other, without one between them that shares less: a lone sequence saves
+// nothing, so it takes any neighbour that it shares 8 pages with. All sequences
+// must be non-null and of one pool (invalid_argument).
 std::vector<PrefixGroup> plan_shared_prefixes(const std::vector<const SequenceState*>& sequences);
 
 // paged_attention_batch (same arguments, checks, exceptions, synchronous
